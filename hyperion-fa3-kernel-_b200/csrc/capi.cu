@@ -21,6 +21,9 @@
 #include "row_mma_kernel.cuh"
 #include "tile_kernel.cuh"
 #include "kv_write.cuh"
+#include "rope_write.cuh"
+#include "key_weights.cuh"
+#include "evict.cuh"
 #include "launch_table.h"
 
 namespace {
@@ -614,6 +617,226 @@ extern "C" int hyperion_kv_cache_write(const void* K_new, const void* V_new, int
   const cudaError_t e = hyp::kvw::launch(a, head_dim, in_dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "cache writer launch");
   return HYPERION_OK;
+}
+
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The checks of the workspace (its error word) that the cache operators share.
+int check_workspace(const void* workspace, size_t workspace_bytes) {
+  if (workspace == nullptr || workspace_bytes < hyp::kWsPartials || !aligned(workspace, 256))
+    return fail(HYPERION_ERR_WORKSPACE, "workspace missing, smaller than 256 bytes or not 256-byte aligned");
+  return HYPERION_OK;
+}
+
+uint32_t* error_word(void* workspace) {
+  return reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + hyp::kWsError);
+}
+
+// The checks of the page layout that the cache operators share.
+int check_pages(const int32_t* tables, int64_t numel, long long rows, int block_size, int num_blocks,
+                long long pool_rows) {
+  if (block_size < 1 || num_blocks < 1) return fail(HYPERION_ERR_INVALID_ARG, "block_size and num_blocks must be >= 1");
+  if (pool_rows < 1) return fail(HYPERION_ERR_INVALID_ARG, "pool_rows < 1");
+  if ((long long)block_size * num_blocks > 0x7fffffffLL)
+    return fail(HYPERION_ERR_UNSUPPORTED, "block_size * num_blocks exceeds int32");
+  if (numel < 0 || (numel > 0 && tables == nullptr))
+    return fail(HYPERION_ERR_INVALID_ARG, "block_tables is NULL but numel > 0");
+  if (numel > 0 && numel < rows * num_blocks)
+    return fail(HYPERION_ERR_INVALID_ARG, "block_tables numel < rows * num_blocks");
+  return HYPERION_OK;
+}
+
+}  // namespace
+
+extern "C" int hyperion_rope_cache_write(const hyperion_rope_write_args* x, void* workspace, size_t workspace_bytes,
+                                         void* stream) {
+  if (x == nullptr) return fail(HYPERION_ERR_INVALID_ARG, "args is NULL");
+  if (x->in_dtype != HYPERION_DTYPE_F16 && x->in_dtype != HYPERION_DTYPE_BF16 && x->in_dtype != HYPERION_DTYPE_F32)
+    return fail(HYPERION_ERR_INVALID_ARG, "in_dtype is not F16, BF16 or F32");
+  if (x->head_dim != 128 && x->head_dim != 256) return fail(HYPERION_ERR_UNSUPPORTED, "head_dim must be 128 or 256");
+  if (x->n_tokens < 0) return fail(HYPERION_ERR_INVALID_ARG, "n_tokens < 0");
+  if (x->n_heads < 1 || x->n_kv_heads < 1) return fail(HYPERION_ERR_INVALID_ARG, "n_heads and n_kv_heads must be >= 1");
+  if (x->rotary_dim < 0 || x->rotary_dim > x->head_dim || x->rotary_dim % 2)
+    return fail(HYPERION_ERR_INVALID_ARG, "rotary_dim must be even and in [0, head_dim]");
+  if (x->layout != HYPERION_ROPE_HALF && x->layout != HYPERION_ROPE_INTERLEAVED)
+    return fail(HYPERION_ERR_INVALID_ARG, "layout must be HYPERION_ROPE_HALF or _INTERLEAVED");
+  if (x->rotary_dim > 0 && x->n_positions < 1) return fail(HYPERION_ERR_INVALID_ARG, "n_positions < 1");
+  if (x->seq_q < 1) return fail(HYPERION_ERR_INVALID_ARG, "seq_q < 1");
+  if (x->q_rows < 0 || x->slot_rows < 0) return fail(HYPERION_ERR_INVALID_ARG, "q_rows or slot_rows < 0");
+  if (x->v_scale_numel < 1) return fail(HYPERION_ERR_INVALID_ARG, "V_scale is empty");
+  int rc = check_pages(x->block_tables, x->block_tables_numel, 0, x->block_size, x->num_blocks, x->pool_rows);
+  if (rc) return rc;
+  rc = check_workspace(workspace, workspace_bytes);
+  if (rc) return rc;
+  if (x->n_tokens == 0) return HYPERION_OK;
+  if (!x->q || !x->k || !x->v || !x->seq_ids || !x->positions || !x->q_words || !x->v_scale || !x->k_cache ||
+      !x->v_cache || (x->rotary_dim > 0 && !x->rope) || (x->slot_rows > 0 && !x->slot_positions))
+    return fail(HYPERION_ERR_INVALID_ARG, "a tensor pointer is NULL");
+  const uintptr_t esz = x->in_dtype == HYPERION_DTYPE_F32 ? 4 : 2;
+  if (!aligned(x->q, esz) || !aligned(x->k, esz) || !aligned(x->v, esz))
+    return fail(HYPERION_ERR_INVALID_ARG, "q, k and v must be aligned to their element size");
+  if (!aligned(x->q_words, 16) || !aligned(x->k_cache, 16) || !aligned(x->v_cache, 16))
+    return fail(HYPERION_ERR_INVALID_ARG, "q_words, k_cache and v_cache must be 16-byte aligned");
+  if ((long long)x->n_tokens * (x->n_heads + (long long)x->n_kv_heads) > 0x7fffffffLL)
+    return fail(HYPERION_ERR_UNSUPPORTED, "too many (token, head) rows");
+  hyp::rope::Args a;
+  a.q = x->q;
+  a.k = x->k;
+  a.v = x->v;
+  a.q_ts = x->q_token_stride;
+  a.q_hs = x->q_head_stride;
+  a.k_ts = x->k_token_stride;
+  a.k_hs = x->k_head_stride;
+  a.v_ts = x->v_token_stride;
+  a.v_hs = x->v_head_stride;
+  a.n_tokens = x->n_tokens;
+  a.n_heads = x->n_heads;
+  a.n_kv_heads = x->n_kv_heads;
+  a.seq_ids = x->seq_ids;
+  a.positions = x->positions;
+  a.q_idx = x->q_idx;
+  a.slots = x->slots;
+  a.slots_per_head = x->slots_per_head;
+  a.table = x->rope;
+  a.n_positions = x->n_positions;
+  a.rot = x->rotary_dim;
+  a.interleaved = x->layout == HYPERION_ROPE_INTERLEAVED;
+  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
+  a.bt_rows = x->block_tables_numel / x->num_blocks;
+  a.block_size = x->block_size;
+  a.num_blocks = x->num_blocks;
+  a.v_scale = x->v_scale;
+  a.v_scale_numel = x->v_scale_numel;
+  a.q_words = x->q_words;
+  a.q_rows = x->q_rows;
+  a.seq_q = x->seq_q;
+  a.k_cache = x->k_cache;
+  a.v_cache = x->v_cache;
+  a.pool_rows = x->pool_rows;
+  a.slot_positions = x->slot_positions;
+  a.slot_rows = x->slot_rows;
+  a.err = error_word(workspace);
+  const cudaError_t e = hyp::rope::launch(a, x->head_dim, x->in_dtype, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "rotary cache writer launch");
+}
+
+extern "C" size_t hyperion_key_weights_scratch_bytes(int32_t n_kv, int32_t kv_group, int32_t n_q, int32_t head_dim,
+                                                     int32_t block_size, int32_t num_blocks) {
+  (void)head_dim;
+  (void)block_size;
+  (void)num_blocks;
+  if (n_kv < 1 || kv_group < 1 || n_q < 1) return 0;
+  return hyp::kweights::scratch_bytes(n_kv, kv_group, n_q);
+}
+
+extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* x, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
+  if (x == nullptr) return fail(HYPERION_ERR_INVALID_ARG, "args is NULL");
+  if (x->head_dim != 128 && x->head_dim != 256) return fail(HYPERION_ERR_UNSUPPORTED, "head_dim must be 128 or 256");
+  if (x->n_kv < 0) return fail(HYPERION_ERR_INVALID_ARG, "n_kv < 0");
+  if (x->kv_group < 1) return fail(HYPERION_ERR_INVALID_ARG, "kv_group < 1");
+  if (x->seq_q < 1 || x->n_q < 1) return fail(HYPERION_ERR_INVALID_ARG, "seq_q and n_q must be >= 1");
+  if (!std::isfinite(x->inv_sqrt_d)) return fail(HYPERION_ERR_INVALID_ARG, "inv_sqrt_d is not finite");
+  if (!std::isfinite(x->decay)) return fail(HYPERION_ERR_INVALID_ARG, "decay is not finite");
+  int rc = check_pages(x->block_tables, x->block_tables_numel, x->n_kv, x->block_size, x->num_blocks, x->pool_rows);
+  if (rc) return rc;
+  if (x->weights_ld < (int64_t)x->block_size * x->num_blocks)
+    return fail(HYPERION_ERR_INVALID_ARG, "weights_ld < num_blocks * block_size");
+  if ((long long)x->n_kv * x->kv_group > 0x7fffffffLL / x->n_q)
+    return fail(HYPERION_ERR_UNSUPPORTED, "too many query rows in the window");
+  rc = check_workspace(workspace, workspace_bytes);
+  if (rc) return rc;
+  if (x->n_kv == 0) return HYPERION_OK;
+  if (!x->q || !x->k_cache || !x->context_lens || !x->weights || !x->weights_out)
+    return fail(HYPERION_ERR_INVALID_ARG, "a tensor pointer is NULL");
+  if (!aligned(x->q, 16) || !aligned(x->k_cache, 16))
+    return fail(HYPERION_ERR_INVALID_ARG, "q and k_cache must be 16-byte aligned");
+  const size_t need = hyperion_key_weights_scratch_bytes(x->n_kv, x->kv_group, x->n_q, x->head_dim, x->block_size,
+                                                         x->num_blocks);
+  if (need > 0 && (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16)))
+    return fail(HYPERION_ERR_WORKSPACE,
+                "scratch missing, smaller than hyperion_key_weights_scratch_bytes() or not 16-byte aligned");
+  hyp::kweights::Args a;
+  a.q = x->q;
+  a.k = x->k_cache;
+  a.ctx_lens = x->context_lens;
+  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
+  a.pool_blocks = x->pool_rows / x->block_size;
+  a.n_kv = x->n_kv;
+  a.kv_group = x->kv_group;
+  a.seq_q = x->seq_q;
+  a.q_first = x->q_first;
+  a.n_q = x->n_q;
+  a.block_size = x->block_size;
+  a.num_blocks = x->num_blocks;
+  a.inv_sqrt_d = x->inv_sqrt_d;
+  a.causal = x->causal ? 1 : 0;
+  a.decay = x->decay;
+  a.in = x->weights;
+  a.out = x->weights_out;
+  a.ld = x->weights_ld;
+  a.stats = static_cast<int2*>(x->scratch);
+  a.err = error_word(workspace);
+  const cudaError_t e = hyp::kweights::launch(a, x->head_dim, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "key weights launch");
+}
+
+extern "C" size_t hyperion_evict_scratch_bytes(int32_t n_kv, int32_t block_size, int32_t num_blocks) {
+  if (n_kv < 1 || block_size < 1 || num_blocks < 1) return 0;
+  return hyp::evict::scratch_bytes(n_kv, block_size, num_blocks);
+}
+
+extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (x == nullptr) return fail(HYPERION_ERR_INVALID_ARG, "args is NULL");
+  if (x->head_dim != 128 && x->head_dim != 256) return fail(HYPERION_ERR_UNSUPPORTED, "head_dim must be 128 or 256");
+  if (x->n_kv < 0) return fail(HYPERION_ERR_INVALID_ARG, "n_kv < 0");
+  if (x->keep_rows == nullptr && x->keep < 0) return fail(HYPERION_ERR_INVALID_ARG, "keep < 0");
+  if (x->sink < 0 || x->recent < 0) return fail(HYPERION_ERR_INVALID_ARG, "sink and recent must be >= 0");
+  int rc = check_pages(x->block_tables, x->block_tables_numel, x->n_kv, x->block_size, x->num_blocks, x->pool_rows);
+  if (rc) return rc;
+  if (x->ld < (int64_t)x->block_size * x->num_blocks)
+    return fail(HYPERION_ERR_INVALID_ARG, "ld < num_blocks * block_size");
+  rc = check_workspace(workspace, workspace_bytes);
+  if (rc) return rc;
+  if (x->n_kv == 0) return HYPERION_OK;
+  if (!x->k_cache || !x->v_cache || !x->context_lens || !x->context_lens_out || !x->weights || !x->weights_out ||
+      !x->positions || !x->positions_out)
+    return fail(HYPERION_ERR_INVALID_ARG, "a tensor pointer is NULL");
+  if (!aligned(x->k_cache, 16) || !aligned(x->v_cache, 16))
+    return fail(HYPERION_ERR_INVALID_ARG, "k_cache and v_cache must be 16-byte aligned");
+  const size_t need = hyperion_evict_scratch_bytes(x->n_kv, x->block_size, x->num_blocks);
+  if (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16))
+    return fail(HYPERION_ERR_WORKSPACE,
+                "scratch missing, smaller than hyperion_evict_scratch_bytes() or not 16-byte aligned");
+  hyp::evict::Args a;
+  a.k = x->k_cache;
+  a.v = x->v_cache;
+  a.v_scale = x->v_scale;
+  a.row_words = x->head_dim / 32;
+  a.ctx_in = x->context_lens;
+  a.ctx_out = x->context_lens_out;
+  a.n_kv = x->n_kv;
+  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
+  a.pool_blocks = x->pool_rows / x->block_size;
+  a.block_size = x->block_size;
+  a.num_blocks = x->num_blocks;
+  a.w_in = x->weights;
+  a.w_out = x->weights_out;
+  a.pos_in = x->positions;
+  a.pos_out = x->positions_out;
+  a.ld = x->ld;
+  a.keep_rows = x->keep_rows;
+  a.keep = x->keep;
+  a.sink = x->sink;
+  a.recent = x->recent;
+  a.holes = static_cast<int32_t*>(x->scratch);
+  a.hole_ld = hyp::evict::hole_ld(x->block_size, x->num_blocks);
+  a.err = error_word(workspace);
+  const cudaError_t e = hyp::evict::launch(a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "eviction launch");
 }
 
 // ---------------------------------------------------------------------------

@@ -61,6 +61,8 @@ _KERNELS = {1: "row", 2: "group", 3: "group_mma", 4: "tile"}
 
 _ws_lock = threading.Lock()
 _workspaces: dict = {}
+_captured: set = set()  # keys of workspaces that a captured graph may hold the address of
+_retired: list = []  # outgrown workspaces of those keys: a graph replays on them
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -71,18 +73,24 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     work counter or split-KV partials, and the calls that use one workspace are
     ordered by its stream.  It is allocated on that stream as well, so when it grows
     the caching allocator hands the old block out again only after the work already
-    queued on the stream."""
+    queued on the stream.  An outgrown block that a call under capture has used is kept:
+    the graph goes on using its address."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     dev = torch.device("cuda", idx)
     key = (idx, torch.cuda.current_stream(dev).cuda_stream)
     with _ws_lock:
         ws = _workspaces.get(key)
+        capturing = torch.cuda.is_current_stream_capturing()
         if ws is None or ws.numel() < nbytes:
             new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev)
             if ws is not None:
                 new[:256].copy_(ws[:256])  # keep the sticky error word
+                if key in _captured:
+                    _retired.append(ws)
             ws = new
             _workspaces[key] = ws
+        if capturing:
+            _captured.add(key)
         return ws
 
 
@@ -390,3 +398,6 @@ def copy_async(dst: int, src: int, nbytes: int, stream=None) -> None:
                                        ctypes.c_void_p(st.cuda_stream))
     if rc != _capi.HYPERION_OK:
         raise RuntimeError(f"hyperion_copy_async failed (status {rc}): {_capi.last_error()}")
+
+
+from .cache import accumulate_key_weights, evict_keys, rope_cache_write  # noqa: E402,F401

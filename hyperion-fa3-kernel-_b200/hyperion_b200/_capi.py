@@ -29,6 +29,9 @@ DTYPE_F16 = 0
 DTYPE_BF16 = 1
 DTYPE_F32 = 2
 
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
+
 PATH_AUTO = 0
 PATH_ROW = 1
 PATH_TILE = 2
@@ -52,6 +55,11 @@ EXPORTED = (
     "hyperion_ipc_close",
     "hyperion_ipc_free",
     "hyperion_copy_async",
+    "hyperion_rope_cache_write",
+    "hyperion_key_weights_scratch_bytes",
+    "hyperion_accumulate_key_weights",
+    "hyperion_evict_scratch_bytes",
+    "hyperion_evict_keys",
 )
 
 IPC_HANDLE_BYTES = 64  # HYPERION_IPC_HANDLE_BYTES
@@ -90,6 +98,52 @@ class Options(ctypes.Structure):
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
+
+
+class RopeWriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("in_dtype", _i32), ("n_tokens", _i32), ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("layout", _i32), ("n_positions", _i32),
+        ("rope", _vp), ("seq_ids", _vp), ("positions", _vp), ("q_idx", _vp), ("slots", _vp),
+        ("slots_per_head", _i32), ("seq_q", _i32),
+        ("q_words", _vp), ("q_rows", _i64),
+        ("block_tables", _vp), ("block_tables_numel", _i64), ("block_size", _i32), ("num_blocks", _i32),
+        ("v_scale", _vp), ("v_scale_numel", _i64),
+        ("k_cache", _vp), ("v_cache", _vp), ("pool_rows", _i64),
+        ("slot_positions", _vp), ("slot_rows", _i64),
+    ]
+
+
+class KeyWeightsArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k_cache", _vp), ("pool_rows", _i64),
+        ("context_lens", _vp), ("block_tables", _vp), ("block_tables_numel", _i64),
+        ("n_kv", _i32), ("kv_group", _i32), ("seq_q", _i32), ("n_q", _i32),
+        ("q_first", _vp),
+        ("head_dim", _i32), ("block_size", _i32), ("num_blocks", _i32), ("causal", _i32),
+        ("inv_sqrt_d", ctypes.c_float), ("decay", ctypes.c_float),
+        ("weights", _vp), ("weights_out", _vp), ("weights_ld", _i64),
+        ("scratch", _vp), ("scratch_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", _vp), ("v_cache", _vp), ("v_scale", _vp), ("pool_rows", _i64),
+        ("head_dim", _i32), ("n_kv", _i32),
+        ("context_lens", _vp), ("context_lens_out", _vp),
+        ("block_tables", _vp), ("block_tables_numel", _i64), ("block_size", _i32), ("num_blocks", _i32),
+        ("weights", _vp), ("weights_out", _vp), ("positions", _vp), ("positions_out", _vp), ("ld", _i64),
+        ("keep_rows", _vp), ("keep", _i32), ("sink", _i32), ("recent", _i32),
+        ("scratch", _vp), ("scratch_bytes", ctypes.c_size_t),
+    ]
+
+
 _FWD_ARGS = [
     _vp, _i32,  # worklist, total_work
     _vp, _vp,  # Q, Q_scale
@@ -130,7 +184,6 @@ def _load() -> ctypes.CDLL:
     lib.hyperion_version.argtypes = []
     lib.hyperion_apex_kernel_noalloc.restype = ctypes.c_int
     lib.hyperion_apex_kernel_noalloc.argtypes = _FWD_ARGS + [_vp]
-    _i64 = ctypes.c_int64
     lib.hyperion_kv_cache_write.restype = ctypes.c_int
     lib.hyperion_kv_cache_write.argtypes = [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64,
                                             _vp, _vp, _i64, _vp, ctypes.c_size_t, _vp]
@@ -147,6 +200,16 @@ def _load() -> ctypes.CDLL:
     lib.hyperion_ipc_free.argtypes = [_vp]
     lib.hyperion_copy_async.restype = ctypes.c_int
     lib.hyperion_copy_async.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_rope_cache_write.restype = ctypes.c_int
+    lib.hyperion_rope_cache_write.argtypes = [ctypes.POINTER(RopeWriteArgs), _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_key_weights_scratch_bytes.restype = ctypes.c_size_t
+    lib.hyperion_key_weights_scratch_bytes.argtypes = [_i32] * 6
+    lib.hyperion_accumulate_key_weights.restype = ctypes.c_int
+    lib.hyperion_accumulate_key_weights.argtypes = [ctypes.POINTER(KeyWeightsArgs), _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_evict_scratch_bytes.restype = ctypes.c_size_t
+    lib.hyperion_evict_scratch_bytes.argtypes = [_i32] * 3
+    lib.hyperion_evict_keys.restype = ctypes.c_int
+    lib.hyperion_evict_keys.argtypes = [ctypes.POINTER(EvictArgs), _vp, ctypes.c_size_t, _vp]
     return lib
 
 

@@ -1,0 +1,292 @@
+"""The steps between the forwards of a bounded cache.
+
+  rope_cache_write        rotary positions on new Q and K, the sign words of both and V's
+                          codes, written where the forward reads them
+  accumulate_key_weights  a running sum of the attention weight of every cached key
+  evict_keys              each cache row cut to a budget by that sum, packed in place
+
+A decode step at the budget is rope_cache_write (slot = the row's context length, then
+length + 1), the forward, accumulate_key_weights, evict_keys.  The three keep the
+forward's conventions: asynchronous on the current stream of the cache's device, arguments
+checked on the host (RuntimeError), bad pages and rows skipped and flagged on the device
+(read_device_errors), cache rows numbered sequence * n_kv_heads + head.  They may be
+captured into CUDA graphs; scratch is allocated per call, so captured graphs share none.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import ctypes
+
+import torch
+
+from . import _capi, _nbytes, _workspace
+
+_IN_DTYPES = {torch.float16: _capi.DTYPE_F16, torch.bfloat16: _capi.DTYPE_BF16, torch.float32: _capi.DTYPE_F32}
+_LAYOUTS = {"half": _capi.ROPE_HALF, "interleaved": _capi.ROPE_INTERLEAVED}
+_WS_BYTES = 1 << 16
+
+
+def _check(cond: bool, name: str, msg: str) -> None:
+    if not cond:
+        raise RuntimeError(f"{name}: {msg}")
+
+
+def _check_device(name: str, dev: torch.device, **tensors) -> None:
+    _check(dev.type == "cuda", name, "the caches must be CUDA tensors")
+    for arg, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{name}: {arg} must be on {dev}")
+
+
+def _check_contiguous(name: str, **tensors) -> None:
+    for arg, t in tensors.items():
+        if t is not None and not t.is_contiguous():
+            raise RuntimeError(f"{name}: {arg} must be contiguous")
+
+
+def _tables(name: str, block_tables: Optional[torch.Tensor]):
+    """(address, numel) of the block tables; (None, 0) for the contiguous layout."""
+    if block_tables is None or block_tables.numel() == 0:
+        return None, 0
+    _check(block_tables.dtype == torch.int32, name, "block_tables must be int32")
+    return block_tables.data_ptr(), block_tables.numel()
+
+
+def _same_or_apart(name: str, arg: str, a: torch.Tensor, b: torch.Tensor) -> None:
+    p, q = a.data_ptr(), b.data_ptr()
+    _check(p == q or p + _nbytes(a) <= q or q + _nbytes(b) <= p, name, f"{arg} overlaps its input")
+
+
+def _call(name: str, fn, args, dev: torch.device, scratch: int = 0) -> None:
+    """Enqueues `fn` on the current stream of `dev`, with fresh scratch where it needs some."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _call(name, fn, args, dev, scratch)
+    if scratch:
+        buf = torch.empty(scratch, dtype=torch.uint8, device=dev)
+        args.scratch, args.scratch_bytes = buf.data_ptr(), scratch
+    ws = _workspace(dev, _WS_BYTES)
+    rc = fn(ctypes.byref(args), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+    if rc != _capi.HYPERION_OK:
+        raise RuntimeError(f"{name} failed (status {rc}): {_capi.last_error()}")
+
+
+def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tensor, seq_ids: torch.Tensor,
+                     positions: torch.Tensor, rope: Optional[torch.Tensor], block_tables: Optional[torch.Tensor],
+                     block_size: int, num_blocks: int, V_scale: torch.Tensor, Q_words: torch.Tensor,
+                     K_cache: torch.Tensor, V_cache: torch.Tensor, *, layout: str = "half", seq_q: int = 1,
+                     q_idx: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                     slot_positions: Optional[torch.Tensor] = None) -> None:
+    """Turns new queries and keys by their positions and writes what the forward reads.
+
+    Q_new [n_tokens, n_heads, head_dim], K_new and V_new [n_tokens, n_kv_heads, head_dim]:
+    float16, bfloat16 or float32, any strides between tokens and heads (slices of a fused
+    projection), each head's dims contiguous.  Token i belongs to sequence seq_ids[i] and
+    stands at positions[i] (int32).
+
+    rope: float32 [n_positions, 2, rotary_dim / 2], the cos and sin row of each position
+    (glue.rope_table); the first rotary_dim dims of a head turn, in the pairs
+    (j, j + rotary_dim / 2) with layout "half" and (2j, 2j + 1) with "interleaved".  None:
+    nothing turns.
+
+    Q_words (int32 storage, head_dim / 32 words a row) gets the sign words of the turned
+    queries at row (seq * n_heads + head) * seq_q + q_idx, the forward's Q; q_idx (int32
+    [n_tokens]) defaults to 0 when seq_q is 1 and to the positions otherwise.  K_cache and
+    V_cache get K's sign words and V's e4m3 codes (as kv_cache_write) at the cache slot
+    slots[i] (int32 [n_tokens] or [n_tokens, n_kv_heads]), by default the position.
+    slot_positions (int32 [cache rows, num_blocks * block_size]) gets the position there.
+
+    A bit is 1 where the exact x*cos - y*sin (or y*cos + x*sin) is >= 0.  Rows, slots,
+    positions and pages out of range are skipped and flagged.  Two tokens of a call must
+    not name the same slot or query row."""
+    name = "rope_cache_write"
+    _check(Q_new.dtype in _IN_DTYPES and K_new.dtype == Q_new.dtype and V_new.dtype == Q_new.dtype, name,
+           "Q_new, K_new and V_new must share a float16, bfloat16 or float32 dtype")
+    _check(Q_new.dim() == 3 and K_new.dim() == 3 and V_new.shape == K_new.shape, name,
+           "Q_new must be [n_tokens, n_heads, head_dim], K_new and V_new [n_tokens, n_kv_heads, head_dim]")
+    n_tokens, n_heads, head_dim = Q_new.shape
+    n_kv = K_new.shape[1]
+    _check(K_new.shape[0] == n_tokens and K_new.shape[2] == head_dim, name, "Q_new and K_new differ in tokens or head_dim")
+    _check(head_dim in (128, 256), name, "head_dim must be 128 or 256")
+    _check(n_heads >= 1 and n_kv >= 1, name, "n_heads and n_kv_heads must be >= 1")
+    qs, ks, vs = Q_new.stride(), K_new.stride(), V_new.stride()
+    _check(n_tokens == 0 or (qs[2] == 1 and ks[2] == 1 and vs[2] == 1), name, "the dims of a head must be contiguous")
+    _check(seq_ids.dtype == torch.int32 and positions.dtype == torch.int32 and seq_ids.numel() == n_tokens
+           and positions.numel() == n_tokens, name, "seq_ids and positions must be int32 [n_tokens]")
+    _check(q_idx is None or (q_idx.dtype == torch.int32 and q_idx.numel() == n_tokens), name,
+           "q_idx must be int32 [n_tokens]")
+    per_head = 0
+    if slots is not None:
+        per_head = 1 if slots.dim() == 2 else 0
+        _check(slots.dtype == torch.int32 and tuple(slots.shape) == ((n_tokens, n_kv) if per_head else (n_tokens,)), name,
+               "slots must be int32 [n_tokens] or [n_tokens, n_kv_heads]")
+    rot = n_pos = 0
+    if rope is not None:
+        _check(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[1] == 2 and rope.shape[0] >= 1, name,
+               "rope must be float32 [n_positions, 2, rotary_dim / 2]")
+        n_pos, rot = rope.shape[0], 2 * rope.shape[2]
+        _check(rot <= head_dim, name, "rope turns more dims than head_dim")
+    _check(layout in _LAYOUTS, name, "layout must be 'half' or 'interleaved'")
+    _check(seq_q >= 1, name, "seq_q must be >= 1")
+    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
+    _check(V_scale.dtype == torch.float32 and V_scale.numel() >= 1, name, "V_scale must be a non-empty float32 tensor")
+    _check(V_cache.element_size() == 1 and V_cache.numel() % head_dim == 0 and V_cache.numel() > 0, name,
+           "V_cache must hold one byte per element, [pool_rows, head_dim]")
+    pool_rows = V_cache.numel() // head_dim
+    _check(_nbytes(K_cache) >= pool_rows * head_dim // 8, name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
+    _check(_nbytes(Q_words) % (head_dim // 8) == 0, name, "Q_words bytes must be a multiple of head_dim/8")
+    slot_rows = 0
+    if slot_positions is not None:
+        _check(slot_positions.dtype == torch.int32 and slot_positions.dim() == 2
+               and slot_positions.shape[1] == block_size * num_blocks, name,
+               "slot_positions must be int32 [cache rows, num_blocks * block_size]")
+        slot_rows = slot_positions.shape[0]
+    bt, bt_numel = _tables(name, block_tables)
+    _check_contiguous(name, seq_ids=seq_ids, positions=positions, rope=rope, block_tables=block_tables, V_scale=V_scale,
+                      Q_words=Q_words, K_cache=K_cache, V_cache=V_cache, q_idx=q_idx, slots=slots,
+                      slot_positions=slot_positions)
+    dev = K_cache.device
+    _check_device(name, dev, Q_new=Q_new, K_new=K_new, V_new=V_new, seq_ids=seq_ids, positions=positions, rope=rope,
+                  block_tables=block_tables, V_scale=V_scale, Q_words=Q_words, V_cache=V_cache, q_idx=q_idx, slots=slots,
+                  slot_positions=slot_positions)
+    args = _capi.RopeWriteArgs(
+        Q_new.data_ptr(), K_new.data_ptr(), V_new.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+        _IN_DTYPES[Q_new.dtype], n_tokens, n_heads, n_kv, head_dim, rot, _LAYOUTS[layout], n_pos,
+        rope.data_ptr() if rot else None, seq_ids.data_ptr(), positions.data_ptr(),
+        None if q_idx is None else q_idx.data_ptr(), None if slots is None else slots.data_ptr(), per_head, seq_q,
+        Q_words.data_ptr(), _nbytes(Q_words) // (head_dim // 8), bt, bt_numel, block_size, num_blocks,
+        V_scale.data_ptr(), V_scale.numel(), K_cache.data_ptr(), V_cache.data_ptr(), pool_rows,
+        slot_positions.data_ptr() if slot_rows else None, slot_rows)
+    _call(name, _capi.lib.hyperion_rope_cache_write, args, dev)
+
+
+def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens: torch.Tensor,
+                           block_tables: Optional[torch.Tensor], weights: torch.Tensor, seq_q: int, head_dim: int,
+                           block_size: int, num_blocks: int, inv_sqrt_d: float, causal: bool, *, kv_group: int = 1,
+                           q_first: Optional[torch.Tensor] = None, n_q: Optional[int] = None, decay: float = 1.0,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adds the attention weight of every cached key, summed over a window of query rows.
+
+    out[r, t] = decay * weights[r, t] + sum of softmax(q . k)[t] over the query rows of
+    cache row r, for t < context_lens[r]; entries beyond are not written.  The weights are
+    the forward's own (clamped softmax, causal: key t is seen by query row i when t <= i).
+    Q, K_cache, context_lens, block_tables, seq_q and kv_group are the forward's.
+
+    The window holds the query rows q_first[r] + i, i < n_q, of each of the row's kv_group
+    query heads (q_first int32 [cache rows], default 0; n_q default seq_q); those outside
+    [0, seq_q) do not count, so q_first = length - 64 with n_q = 64 takes the last 64 rows
+    of every prompt, all rows of a shorter one.
+
+    weights: float32 [cache rows, >= num_blocks * block_size]; out: as weights, weights
+    itself by default.  Returns out.  The same inputs give the same bits."""
+    name = "accumulate_key_weights"
+    _check(head_dim in (128, 256), name, "head_dim must be 128 or 256")
+    _check(context_lens.dtype == torch.int32, name, "context_lens must be int32")
+    n_kv = context_lens.numel()
+    n_q = seq_q if n_q is None else n_q
+    _check(kv_group >= 1 and seq_q >= 1 and n_q >= 1, name, "kv_group, seq_q and n_q must be >= 1")
+    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
+    row_bytes = head_dim // 8
+    _check(_nbytes(Q) >= n_kv * kv_group * seq_q * row_bytes, name, "Q smaller than its rows of head_dim/8 bytes")
+    _check(_nbytes(K_cache) % row_bytes == 0 and K_cache.numel() > 0, name, "K_cache must be [pool_rows, head_dim/32] words")
+    out = weights if out is None else out
+    for arg, t in (("weights", weights), ("out", out)):
+        _check(t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == n_kv
+               and t.shape[1] >= block_size * num_blocks, name,
+               f"{arg} must be float32 [cache rows, >= num_blocks * block_size]")
+    _check(out.shape == weights.shape, name, "out must have the shape of weights")
+    _check(q_first is None or (q_first.dtype == torch.int32 and q_first.numel() == n_kv), name,
+           "q_first must be int32 [cache rows]")
+    bt, bt_numel = _tables(name, block_tables)
+    _check(bt_numel == 0 or bt_numel >= n_kv * num_blocks, name, "block_tables numel < cache rows * num_blocks")
+    _check_contiguous(name, Q=Q, K_cache=K_cache, context_lens=context_lens, block_tables=block_tables, weights=weights,
+                      out=out, q_first=q_first)
+    if out is not weights:
+        _same_or_apart(name, "out", weights, out)
+    dev = K_cache.device
+    _check_device(name, dev, Q=Q, context_lens=context_lens, block_tables=block_tables, weights=weights, out=out,
+                  q_first=q_first)
+    if n_kv == 0:
+        return out
+    args = _capi.KeyWeightsArgs(
+        Q.data_ptr(), K_cache.data_ptr(), _nbytes(K_cache) // row_bytes, context_lens.data_ptr(), bt, bt_numel, n_kv,
+        kv_group, seq_q, n_q, None if q_first is None else q_first.data_ptr(), head_dim, block_size, num_blocks,
+        1 if causal else 0, inv_sqrt_d, decay, weights.data_ptr(), out.data_ptr(), weights.shape[1])
+    _call(name, _capi.lib.hyperion_accumulate_key_weights, args, dev,
+          _capi.lib.hyperion_key_weights_scratch_bytes(n_kv, kv_group, n_q, head_dim, block_size, num_blocks))
+    return out
+
+
+def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch.Tensor,
+               block_tables: Optional[torch.Tensor], block_size: int, num_blocks: int, weights: torch.Tensor,
+               positions: torch.Tensor, keep: Union[int, torch.Tensor], *, sink: int = 0, recent: int = 0,
+               V_scale: Optional[torch.Tensor] = None, context_lens_out: Optional[torch.Tensor] = None,
+               weights_out: Optional[torch.Tensor] = None,
+               positions_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cuts every cache row to its budget, in place.
+
+    Of the n = context_lens[r] keys of row r the m = min(n, keep) highest-ranked stay
+    (keep: an int, or int32 [cache rows]).  Keys at a position below `sink` or among the
+    last `recent` positions up to the row's newest rank above all others; the others rank
+    by weights (float32 [cache rows, >= num_blocks * block_size], the sums of
+    accumulate_key_weights; NaN lowest); equal ranks go to the lower slot.
+
+    Slots are not shifted: the i-th slot below m whose key goes takes the i-th kept key at
+    or beyond m, so a step that drops one key moves at most one.  K words, V codes, the
+    per-slot V_scale where one is given (float32 [pool rows]; other scales do not move),
+    weights and positions (int32, as weights: each slot's position, as rope_cache_write's
+    slot_positions) move together.  Slots m <= t < n end with weight 0 and position -1,
+    ready for the next keys.  Pages beyond ceil(m / block_size) of a row are free to go.
+
+    The new lengths, weights and positions go to the *_out tensors, by default the inputs
+    themselves.  Returns the new lengths (context_lens_out).  Rows must not share pages."""
+    name = "evict_keys"
+    _check(V_cache.element_size() == 1 and V_cache.dim() == 2 and V_cache.shape[1] in (128, 256) and V_cache.shape[0] > 0,
+           name, "V_cache must hold one byte per element, [pool_rows, head_dim] with head_dim 128 or 256")
+    pool_rows, head_dim = V_cache.shape
+    _check(_nbytes(K_cache) >= pool_rows * head_dim // 8, name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
+    _check(context_lens.dtype == torch.int32, name, "context_lens must be int32")
+    n_kv = context_lens.numel()
+    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
+    ctx_out = context_lens if context_lens_out is None else context_lens_out
+    w_out = weights if weights_out is None else weights_out
+    p_out = positions if positions_out is None else positions_out
+    _check(ctx_out.dtype == torch.int32 and ctx_out.numel() == n_kv, name, "context_lens_out must be int32 [cache rows]")
+    for arg, t, dt in (("weights", weights, torch.float32), ("weights_out", w_out, torch.float32),
+                       ("positions", positions, torch.int32), ("positions_out", p_out, torch.int32)):
+        _check(t.dtype == dt and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks
+               and t.shape == weights.shape, name,
+               f"{arg} must be {str(dt)[6:]} [cache rows, >= num_blocks * block_size], all four of one shape")
+    keep_rows = keep if isinstance(keep, torch.Tensor) else None
+    if keep_rows is not None:
+        _check(keep.dtype == torch.int32 and keep.numel() == n_kv, name, "keep must be an int or int32 [cache rows]")
+    else:
+        _check(keep >= 0, name, "keep must be >= 0")
+        keep = min(keep, 0x7FFFFFFF)
+    _check(0 <= sink <= 0x7FFFFFFF and 0 <= recent <= 0x7FFFFFFF, name, "sink and recent must be >= 0 and fit int32")
+    _check(V_scale is None or (V_scale.dtype == torch.float32 and V_scale.numel() == pool_rows), name,
+           "V_scale must be float32 [pool_rows], one scale per slot; other scales do not move")
+    bt, bt_numel = _tables(name, block_tables)
+    _check(bt_numel == 0 or bt_numel >= n_kv * num_blocks, name, "block_tables numel < cache rows * num_blocks")
+    _check_contiguous(name, K_cache=K_cache, V_cache=V_cache, context_lens=context_lens, block_tables=block_tables,
+                      weights=weights, positions=positions, keep=keep_rows, V_scale=V_scale, context_lens_out=ctx_out,
+                      weights_out=w_out, positions_out=p_out)
+    for arg, a, b in (("context_lens_out", context_lens, ctx_out), ("weights_out", weights, w_out),
+                      ("positions_out", positions, p_out)):
+        if a is not b:
+            _same_or_apart(name, arg, a, b)
+    dev = K_cache.device
+    _check_device(name, dev, V_cache=V_cache, context_lens=context_lens, block_tables=block_tables, weights=weights,
+                  positions=positions, keep=keep_rows, V_scale=V_scale, context_lens_out=ctx_out, weights_out=w_out,
+                  positions_out=p_out)
+    if n_kv == 0:
+        return ctx_out
+    args = _capi.EvictArgs(
+        K_cache.data_ptr(), V_cache.data_ptr(), None if V_scale is None else V_scale.data_ptr(), pool_rows, head_dim, n_kv,
+        context_lens.data_ptr(), ctx_out.data_ptr(), bt, bt_numel, block_size, num_blocks, weights.data_ptr(),
+        w_out.data_ptr(), positions.data_ptr(), p_out.data_ptr(), weights.shape[1],
+        None if keep_rows is None else keep_rows.data_ptr(), 0 if keep_rows is not None else keep, sink, recent)
+    _call(name, _capi.lib.hyperion_evict_keys, args, dev,
+          _capi.lib.hyperion_evict_scratch_bytes(n_kv, block_size, num_blocks))
+    return ctx_out

@@ -13,6 +13,7 @@
 """
 from __future__ import annotations
 
+import math
 import zlib
 from typing import Dict, Optional, Sequence, Tuple
 
@@ -102,3 +103,41 @@ def memory_requirements(model_size_b: float, context_len: int, batch_size: int, 
         "fits_on_3090": total_gb < 24.0,
         "fits_on_b200": total_gb < 180.0,
     }
+
+
+def rope_table(n_positions: int, rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None,
+               factor: float = 1.0, original_positions: int = 0, low_turns: float = 1.0, high_turns: float = 32.0,
+               device=None) -> torch.Tensor:
+    """The cos / sin table of rope_cache_write: float32 [n_positions, 2, rotary_dim / 2].
+
+    Row p holds cos(p f_j) and sin(p f_j), f_j = base^(-2j / rotary_dim), angles in 64 bits
+    and each value rounded once, so far positions keep their angles.  `scaling` fits a
+    context `factor` times the one the base was trained for:
+      None      the plain frequencies;
+      "linear"  f_j / factor (every position scaled down);
+      "base"    base * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair is slowed by
+                the factor, the fastest not at all;
+      "bands"   pairs that turn more than high_turns times over original_positions stay,
+                those that turn less than low_turns times are divided by the factor, those
+                between go linearly from one to the other in their number of turns."""
+    if n_positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("n_positions must be >= 1 and rotary_dim even and >= 2")
+    if not base > 0 or not factor > 0:
+        raise ValueError("base and factor must be > 0")
+    if scaling not in (None, "linear", "base", "bands"):
+        raise ValueError("scaling must be None, 'linear', 'base' or 'bands'")
+    if scaling == "base":
+        if rotary_dim < 4:
+            raise ValueError("scaling 'base' needs rotary_dim >= 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "bands":
+        if original_positions < 1 or not high_turns > low_turns:
+            raise ValueError("scaling 'bands' needs original_positions >= 1 and high_turns > low_turns")
+        turns = original_positions * freq / (2 * math.pi)
+        stay = ((turns - low_turns) / (high_turns - low_turns)).clamp(0, 1)
+        freq = freq * stay + freq / factor * (1 - stay)
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.stack([angle.cos(), angle.sin()], dim=1).to(torch.float32)

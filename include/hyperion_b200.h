@@ -255,6 +255,146 @@ int hyperion_kv_cache_write(const void* K_new, const void* V_new, int32_t in_dty
                             uint32_t* K_cache, uint8_t* V_cache, int64_t pool_rows,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* Rotary positions on new queries and keys, fused with the packing of both and the cache
+ * write: what stands between a layer's projections and the forward.  It has no counterpart
+ * in the reference.
+ *
+ * For each token i (position p = positions[i], sequence b = seq_ids[i]) and head:
+ *   dims below rotary_dim turn in pairs by the table's row p (cos[rotary_dim/2], then
+ *   sin[rotary_dim/2]):  r_a = x_a cos - x_b sin,  r_b = x_b cos + x_a sin;
+ *   pair j is dims (j, j + rotary_dim/2) with HYPERION_ROPE_HALF and (2j, 2j + 1) with
+ *   HYPERION_ROPE_INTERLEAVED; dims from rotary_dim on pass through.
+ * Q: sign bits (1 where r >= 0) to row (b*n_heads + h)*seq_q + q_idx[i] of q_words, the
+ *    forward's Q layout; q_idx NULL stands for 0 when seq_q is 1 and for p otherwise.
+ * K: sign bits to slot slots[i] of cache row b*n_kv_heads + h (the paged or contiguous
+ *    layout of the forward); slots NULL stands for p.  A cache that has been through
+ *    hyperion_evict_keys has slots that are not positions.
+ * V: e4m3 codes as hyperion_kv_cache_write writes them, to the same slot.
+ * slot_positions, where given, gets p at [cache row, slot].
+ * The sign is that of the exact sum of the two products, for f32 table values and inputs
+ * of any of the three types, whatever the sum's rounding would be.  NaN gives bit 0.
+ * A token with a negative sequence, a position outside the table, or rows or slots outside
+ * Q, the tables or slot_positions sets HYPERION_DEVERR_BAD_ITEM, a page outside the pool
+ * HYPERION_DEVERR_BAD_BLOCK; what they concern is skipped.  Two tokens of a call must not
+ * name the same slot or Q row.  The inputs must not overlap the outputs. */
+#define HYPERION_ROPE_HALF         0
+#define HYPERION_ROPE_INTERLEAVED  1
+
+typedef struct hyperion_rope_write_args {
+  const void* q;            /* [n_tokens, n_heads, head_dim] of in_dtype */
+  const void* k;            /* [n_tokens, n_kv_heads, head_dim] */
+  const void* v;            /* [n_tokens, n_kv_heads, head_dim] */
+  int64_t q_token_stride, q_head_stride;  /* in elements; a head's dims are contiguous */
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int32_t in_dtype;         /* HYPERION_DTYPE_* */
+  int32_t n_tokens, n_heads, n_kv_heads, head_dim;
+  int32_t rotary_dim;       /* even, 0..head_dim; 0: nothing turns and rope may be NULL */
+  int32_t layout;           /* HYPERION_ROPE_* */
+  int32_t n_positions;      /* rows of rope */
+  const float* rope;        /* [n_positions, 2, rotary_dim / 2]: cos row, sin row */
+  const int32_t* seq_ids;   /* [n_tokens] */
+  const int32_t* positions; /* [n_tokens] */
+  const int32_t* q_idx;     /* [n_tokens] or NULL */
+  const int32_t* slots;     /* [n_tokens], [n_tokens, n_kv_heads] or NULL */
+  int32_t slots_per_head;   /* 1: slots is [n_tokens, n_kv_heads] */
+  int32_t seq_q;            /* query rows per (sequence, head) of q_words */
+  uint32_t* q_words;        /* [q_rows, head_dim / 32] */
+  int64_t q_rows;
+  const int32_t* block_tables;
+  int64_t block_tables_numel;  /* 0: contiguous layout */
+  int32_t block_size, num_blocks;
+  const float* v_scale;     /* per tensor, per slot or per head, as in the forward */
+  int64_t v_scale_numel;
+  uint32_t* k_cache;        /* [pool_rows, head_dim / 32] */
+  uint8_t* v_cache;         /* [pool_rows, head_dim] */
+  int64_t pool_rows;
+  int32_t* slot_positions;  /* [slot_rows, num_blocks * block_size] or NULL */
+  int64_t slot_rows;
+} hyperion_rope_write_args;
+
+int hyperion_rope_cache_write(const hyperion_rope_write_args* args, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Adds to a running sum per cached key the attention weight it receives from a window of
+ * query rows: the forward's softmax weights, which the forward does not write.  It has no
+ * counterpart in the reference.  For cache row r, t < n = context_lens[r]:
+ *   weights_out[r, t] = decay * weights[r, t] + sum_q w_q[t]
+ * over the query rows q = (r*kv_group + g)*seq_q + i, g < kv_group, i in
+ * [q_first[r], q_first[r] + n_q) and in [0, seq_q) (q_first NULL: 0), with
+ *   w_q[t] = exp(max(s_t - max s, -80)) / sum of the same over the keys q sees,
+ *   s_t = (head_dim - 2*popcount(q XOR k_t)) * inv_sqrt_d;
+ * q sees the keys t < n, and t <= i when causal; a row that sees none adds nothing.  Keys
+ * on a page outside the pool are left out (HYPERION_DEVERR_BAD_BLOCK), context lengths are
+ * clamped and flagged as in the forward.  Entries t >= n of weights_out are not written.
+ * weights_out is weights itself or does not overlap it.  The sum's order is fixed: the
+ * same inputs give the same bits.
+ * `scratch`: device memory of hyperion_key_weights_scratch_bytes() bytes, 16-byte aligned,
+ * that no other call in flight uses (0 bytes: may be NULL). */
+typedef struct hyperion_key_weights_args {
+  const uint32_t* q;         /* [n_kv * kv_group * seq_q, head_dim / 32] */
+  const uint32_t* k_cache;   /* [pool_rows, head_dim / 32] */
+  int64_t pool_rows;
+  const int32_t* context_lens;  /* [n_kv] */
+  const int32_t* block_tables;
+  int64_t block_tables_numel;
+  int32_t n_kv, kv_group, seq_q, n_q;
+  const int32_t* q_first;    /* [n_kv] or NULL */
+  int32_t head_dim, block_size, num_blocks;
+  int32_t causal;
+  float inv_sqrt_d, decay;
+  const float* weights;      /* [n_kv, weights_ld] */
+  float* weights_out;        /* [n_kv, weights_ld] */
+  int64_t weights_ld;        /* >= num_blocks * block_size */
+  void* scratch;
+  size_t scratch_bytes;
+} hyperion_key_weights_args;
+
+size_t hyperion_key_weights_scratch_bytes(int32_t n_kv, int32_t kv_group, int32_t n_q, int32_t head_dim,
+                                          int32_t block_size, int32_t num_blocks);
+int hyperion_accumulate_key_weights(const hyperion_key_weights_args* args, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* Cuts every cache row to its budget, in place: of the n = context_lens[r] keys of row r the
+ * m = min(n, budget) highest-ranked stay (a negative budget counts as 0).  It has no
+ * counterpart in the reference.  A key is protected when its position is below `sink` or
+ * above (the greatest position of the row's keys) - `recent`; protected keys rank above all
+ * others, the others by `weights` (NaN lowest, -0 as 0), equal ranks by the lower slot.
+ * The i-th slot below m whose key goes takes the i-th kept key at or beyond m: K words, V
+ * codes, the per-slot V scale where v_scale is given, its weight and its position.  Kept
+ * keys below m stay where they are, so slots are not in the order of positions afterwards;
+ * positions[] carries each slot's own.
+ *   context_lens_out[r] = m;  weights_out / positions_out[r, t]: the new row for t < m, then
+ *   0 / -1 for m <= t < n; entries t >= n are not written.
+ * Each of the three outputs is its input itself or does not overlap it.  Rows share no pages.
+ * A move from or to a page outside the pool leaves K and V alone
+ * (HYPERION_DEVERR_BAD_BLOCK); context lengths are clamped and flagged as in the forward.
+ * `scratch`: as above, hyperion_evict_scratch_bytes() bytes. */
+typedef struct hyperion_evict_args {
+  uint32_t* k_cache;         /* [pool_rows, head_dim / 32] */
+  uint8_t* v_cache;          /* [pool_rows, head_dim] */
+  float* v_scale;            /* [pool_rows] where the scale is per slot, else NULL */
+  int64_t pool_rows;
+  int32_t head_dim, n_kv;
+  const int32_t* context_lens;  /* [n_kv] */
+  int32_t* context_lens_out;
+  const int32_t* block_tables;
+  int64_t block_tables_numel;
+  int32_t block_size, num_blocks;
+  const float* weights;      /* [n_kv, ld] */
+  float* weights_out;
+  const int32_t* positions;  /* [n_kv, ld] */
+  int32_t* positions_out;
+  int64_t ld;                /* >= num_blocks * block_size */
+  const int32_t* keep_rows;  /* [n_kv] budgets, or NULL: `keep` for every row */
+  int32_t keep, sink, recent;
+  void* scratch;
+  size_t scratch_bytes;
+} hyperion_evict_args;
+
+size_t hyperion_evict_scratch_bytes(int32_t n_kv, int32_t block_size, int32_t num_blocks);
+int hyperion_evict_keys(const hyperion_evict_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Fixed scratch of hyperion_apex_kernel_noalloc, per device, in bytes. */
 #define HYPERION_NOALLOC_SCRATCH_BYTES ((size_t)32 << 20)
 

@@ -639,8 +639,8 @@ int check_pages(const int32_t* tables, int64_t numel, long long rows, int block_
                 long long pool_rows) {
   if (block_size < 1 || num_blocks < 1) return fail(HYPERION_ERR_INVALID_ARG, "block_size and num_blocks must be >= 1");
   if (pool_rows < 1) return fail(HYPERION_ERR_INVALID_ARG, "pool_rows < 1");
-  if ((long long)block_size * num_blocks > 0x7fffffffLL)
-    return fail(HYPERION_ERR_UNSUPPORTED, "block_size * num_blocks exceeds int32");
+  if ((long long)block_size * num_blocks > 0x7fff0000LL)  // the kernels' key indices are int32, a block ahead at most
+    return fail(HYPERION_ERR_UNSUPPORTED, "block_size * num_blocks exceeds 0x7fff0000");
   if (numel < 0 || (numel > 0 && tables == nullptr))
     return fail(HYPERION_ERR_INVALID_ARG, "block_tables is NULL but numel > 0");
   if (numel > 0 && numel < rows * num_blocks)
@@ -703,10 +703,8 @@ extern "C" int hyperion_rope_cache_write(const hyperion_rope_write_args* x, void
   a.n_positions = x->n_positions;
   a.rot = x->rotary_dim;
   a.interleaved = x->layout == HYPERION_ROPE_INTERLEAVED;
-  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
+  a.pages = hyp::Pages(x->block_tables, x->block_tables_numel, x->block_size, x->num_blocks, x->pool_rows);
   a.bt_rows = x->block_tables_numel / x->num_blocks;
-  a.block_size = x->block_size;
-  a.num_blocks = x->num_blocks;
   a.v_scale = x->v_scale;
   a.v_scale_numel = x->v_scale_numel;
   a.q_words = x->q_words;
@@ -718,17 +716,19 @@ extern "C" int hyperion_rope_cache_write(const hyperion_rope_write_args* x, void
   a.slot_positions = x->slot_positions;
   a.slot_rows = x->slot_rows;
   a.err = error_word(workspace);
-  const cudaError_t e = hyp::rope::launch(a, x->head_dim, x->in_dtype, static_cast<cudaStream_t>(stream));
+  const DevInfo* di = nullptr;
+  rc = get_dev(&di);
+  if (rc) return rc;
+  const cudaError_t e = hyp::rope::launch(a, x->head_dim, x->in_dtype, di->n_sm, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "rotary cache writer launch");
 }
 
 extern "C" size_t hyperion_key_weights_scratch_bytes(int32_t n_kv, int32_t kv_group, int32_t n_q, int32_t head_dim,
                                                      int32_t block_size, int32_t num_blocks) {
-  (void)head_dim;
-  (void)block_size;
-  (void)num_blocks;
-  if (n_kv < 1 || kv_group < 1 || n_q < 1) return 0;
-  return hyp::kweights::scratch_bytes(n_kv, kv_group, n_q);
+  if (n_kv < 1 || kv_group < 1 || n_q < 1 || block_size < 1 || num_blocks < 1) return 0;
+  const hyp::kweights::Plan p =
+      hyp::kweights::plan(n_kv, (long long)kv_group * n_q, head_dim, (long long)block_size * num_blocks);
+  return p.dist_bytes + p.part_bytes;
 }
 
 extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* x, void* workspace,
@@ -744,6 +744,7 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
   if (rc) return rc;
   if (x->weights_ld < (int64_t)x->block_size * x->num_blocks)
     return fail(HYPERION_ERR_INVALID_ARG, "weights_ld < num_blocks * block_size");
+  if (x->pool_rows > 0xffffffffLL) return fail(HYPERION_ERR_UNSUPPORTED, "pool_rows exceeds 32 bits");
   if ((long long)x->n_kv * x->kv_group > 0x7fffffffLL / x->n_q)
     return fail(HYPERION_ERR_UNSUPPORTED, "too many query rows in the window");
   rc = check_workspace(workspace, workspace_bytes);
@@ -753,33 +754,34 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
     return fail(HYPERION_ERR_INVALID_ARG, "a tensor pointer is NULL");
   if (!aligned(x->q, 16) || !aligned(x->k_cache, 16))
     return fail(HYPERION_ERR_INVALID_ARG, "q and k_cache must be 16-byte aligned");
-  const size_t need = hyperion_key_weights_scratch_bytes(x->n_kv, x->kv_group, x->n_q, x->head_dim, x->block_size,
-                                                         x->num_blocks);
-  if (need > 0 && (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16)))
-    return fail(HYPERION_ERR_WORKSPACE,
-                "scratch missing, smaller than hyperion_key_weights_scratch_bytes() or not 16-byte aligned");
+  if (!aligned(x->weights, 4) || !aligned(x->weights_out, 4))
+    return fail(HYPERION_ERR_INVALID_ARG, "weights and weights_out must be aligned to their element size");
+  if (x->scratch == nullptr || !aligned(x->scratch, 16))
+    return fail(HYPERION_ERR_WORKSPACE, "scratch missing or not 16-byte aligned");
+  const hyp::kweights::Plan p = hyp::kweights::plan(x->n_kv, (long long)x->kv_group * x->n_q, x->head_dim,
+                                                    (long long)x->block_size * x->num_blocks);
+  if (x->scratch_bytes < p.dist_bytes + p.part_bytes)
+    return fail(HYPERION_ERR_WORKSPACE, "scratch smaller than hyperion_key_weights_scratch_bytes()");
   hyp::kweights::Args a;
   a.q = x->q;
   a.k = x->k_cache;
   a.ctx_lens = x->context_lens;
-  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
-  a.pool_blocks = x->pool_rows / x->block_size;
+  a.pages = hyp::Pages(x->block_tables, x->block_tables_numel, x->block_size, x->num_blocks, x->pool_rows);
   a.n_kv = x->n_kv;
   a.kv_group = x->kv_group;
   a.seq_q = x->seq_q;
   a.q_first = x->q_first;
   a.n_q = x->n_q;
-  a.block_size = x->block_size;
-  a.num_blocks = x->num_blocks;
   a.inv_sqrt_d = x->inv_sqrt_d;
   a.causal = x->causal ? 1 : 0;
   a.decay = x->decay;
   a.in = x->weights;
   a.out = x->weights_out;
   a.ld = x->weights_ld;
-  a.stats = static_cast<int2*>(x->scratch);
+  a.stats = nullptr;
   a.err = error_word(workspace);
-  const cudaError_t e = hyp::kweights::launch(a, x->head_dim, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = hyp::kweights::launch(a, x->head_dim, static_cast<uint8_t*>(x->scratch),
+                                              static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "key weights launch");
 }
 
@@ -819,10 +821,7 @@ extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace
   a.ctx_in = x->context_lens;
   a.ctx_out = x->context_lens_out;
   a.n_kv = x->n_kv;
-  a.block_tables = x->block_tables_numel > 0 ? x->block_tables : nullptr;
-  a.pool_blocks = x->pool_rows / x->block_size;
-  a.block_size = x->block_size;
-  a.num_blocks = x->num_blocks;
+  a.pages = hyp::Pages(x->block_tables, x->block_tables_numel, x->block_size, x->num_blocks, x->pool_rows);
   a.w_in = x->weights;
   a.w_out = x->weights_out;
   a.pos_in = x->positions;

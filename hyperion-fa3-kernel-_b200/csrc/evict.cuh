@@ -11,7 +11,7 @@
 // never meet.
 #pragma once
 
-#include "common.cuh"
+#include "cache_pages.cuh"
 
 namespace hyp {
 namespace evict {
@@ -27,9 +27,7 @@ struct Args {
   const int32_t* ctx_in;
   int32_t* ctx_out;
   int n_kv;
-  const int32_t* block_tables;
-  long long pool_blocks;
-  int block_size, num_blocks;
+  Pages pages;
   const float* w_in;
   float* w_out;
   const int32_t* pos_in;
@@ -47,14 +45,6 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   if (w != w) return 0;
   const uint32_t b = __float_as_uint(w + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
-__device__ __forceinline__ long long slot_of(const Args& a, int r, int t) {
-  const int page = t / a.block_size;
-  const long long id = a.block_tables ? (long long)__ldg(a.block_tables + (long long)r * a.num_blocks + page)
-                                      : (long long)r * a.num_blocks + page;
-  if (id < 0 || id >= a.pool_blocks) return -1;
-  return id * a.block_size + (t - page * a.block_size);
 }
 
 // Sum of `x` over the lower-numbered threads of the block; *total gets the whole sum.
@@ -83,11 +73,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(Args a) {
   __shared__ int s_warp[kThreads / 32];
   __shared__ int s_pick[2];
   const int r = blockIdx.x, tid = threadIdx.x;
-  const long long cap = (long long)a.num_blocks * a.block_size;
-  int n = a.ctx_in[r];
-  if (tid == 0 && n < 0) raise_error(a.err, HYPERION_DEVERR_NEG_CTX);
-  if (tid == 0 && (long long)n > cap) raise_error(a.err, HYPERION_DEVERR_CTX_OVERFLOW);
-  n = n < 0 ? 0 : (long long)n > cap ? (int)cap : n;
+  const int n = a.pages.context(a.ctx_in[r], a.err, tid == 0);
   int m = a.keep_rows ? __ldg(a.keep_rows + r) : a.keep;
   m = min(n, max(m, 0));
   const float* w = a.w_in + r * a.ld;
@@ -166,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(Args a) {
       const int to = holes[sr];
       w_out[to] = w[t];
       pos_out[to] = pos[t];
-      const long long src = slot_of(a, r, t), dst = slot_of(a, r, to);
+      const long long src = a.pages.slot(r, t), dst = a.pages.slot(r, to);
       if (src < 0 || dst < 0) {
         raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
       } else {

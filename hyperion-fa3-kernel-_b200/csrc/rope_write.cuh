@@ -10,12 +10,19 @@
 // e4m3 codes as in kv_write.cuh.
 #pragma once
 
+#include <algorithm>
+
+#include "cache_pages.cuh"
 #include "kv_write.cuh"
 
 namespace hyp {
 namespace rope {
 
 constexpr int kWarpsPerBlock = 8;
+// Query rows of one lane group in flight at once: 4 rows of 16-bit values are 128 bytes a
+// thread, enough in flight to cover HBM's latency at the kernel's occupancy.
+template <typename T>
+constexpr int kUnroll = sizeof(T) == 2 ? 4 : 2;
 
 struct Args {
   const void* q;  // [n_tokens, n_heads, D], strides in elements
@@ -30,9 +37,8 @@ struct Args {
   int slots_per_head;
   const float* table;  // [n_positions, 2, rot / 2]: cos row, sin row
   int n_positions, rot, interleaved;
-  const int32_t* block_tables;
+  Pages pages;
   long long bt_rows;
-  int block_size, num_blocks;
   const float* v_scale;
   long long v_scale_numel;
   uint32_t* q_words;
@@ -56,8 +62,251 @@ __device__ __forceinline__ bool sum_is_nonneg(float x, float c, float y, float s
   return __dadd_rn(__dmul_rn((double)x, (double)c), __dmul_rn((double)y, (double)s)) >= 0.0;
 }
 
-// One warp per (token, head) of Q and per (token, KV head) of K and V.  Lane l takes
-// dims l, l + 32, ..., so a ballot is one sign word.
+// Query row of (sequence b, head h) for token `tok` at `pos`, or -1.
+__device__ __forceinline__ long long q_row_of(const Args& a, int tok, int b, int pos, int h) {
+  const int qi = a.q_idx ? __ldg(a.q_idx + tok) : (a.seq_q == 1 ? 0 : pos);
+  const long long row = ((long long)b * a.n_heads + h) * a.seq_q + qi;
+  return qi < 0 || qi >= a.seq_q || row >= a.q_rows ? -1 : row;
+}
+
+// Pool row of cache row kv for token `tok` at `pos`, or -1 with the error raised by `flag`.
+__device__ __forceinline__ long long kv_row_of(const Args& a, int tok, int pos, int h, long long kv, bool flag, int* slot) {
+  const int t = a.slots ? __ldg(a.slots + (a.slots_per_head ? (long long)tok * a.n_kv_heads + h : (long long)tok)) : pos;
+  *slot = t;
+  if (t < 0 || t >= a.pages.capacity() || (a.pages.tables && kv >= a.bt_rows) ||
+      (a.slot_positions && kv >= a.slot_rows)) {
+    if (flag) raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
+    return -1;
+  }
+  const long long row = a.pages.slot(kv, t);
+  if (row < 0 && flag) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+  return row;
+}
+
+__device__ __forceinline__ float v_scale_of(const Args& a, long long kv, long long row) {
+  const long long si = a.v_scale_numel == 1 ? 0 : (a.v_scale_numel == a.pool_rows ? row : kv % a.v_scale_numel);
+  return __ldg(a.v_scale + si);
+}
+
+__device__ __forceinline__ uint32_t v_code(float v, float scale) {
+  float y = __fdiv_rn(v, scale);
+  if (y == y) y = fminf(fmaxf(y, -448.f), 448.f);
+  return kvw::e4m3_code(y);
+}
+
+// ---------------------------------------------------------------------------
+// The vector kernel: rotary_dim a multiple of 16, inputs on 16-byte boundaries.
+//
+// D / 16 lanes share a row, so a warp holds 4 rows of 128 dims or 2 of 256.  Lane j of a
+// row takes 16 dims as two runs of 8, each one 16-byte load of 16-bit values and one byte
+// of signs: the run of pair members a and that of members b (half layout), or 16
+// neighbouring dims (interleaved).  Either way its pairs are 8j .. 8j + 7, and the warp
+// keeps one token's cos / sin in registers for all the heads it takes.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Run8 {
+  uint4 x[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Run8<T> load8(const T* p) {
+  Run8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.x[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen8(const Run8<T>& r, float (&f)[8]) {
+  const T* p = reinterpret_cast<const T*>(r.x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = kvw::to_f32<T>(p[i]);
+}
+
+// Signs of x*c + y*s for 8 elements as a byte (element 0 in bit 0, 1 where >= 0).  The
+// sign bits of the rounded sums are shifted in one by one; a sum that is zero or NaN sends
+// the run to the exact form.
+__device__ __forceinline__ uint32_t sign_byte(const float (&x)[8], const float (&c)[8], const float (&y)[8],
+                                              const float (&s)[8], bool minus) {
+  uint32_t neg = 0;
+  bool clear = true;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float u = __fmul_rn(x[i], c[i]), w = __fmul_rn(y[i], s[i]);
+    const float d = minus ? __fsub_rn(u, w) : __fadd_rn(u, w);
+    neg = __funnelshift_l(__float_as_uint(d), neg, 1);
+    clear = clear && fabsf(d) > 0.f;
+  }
+  uint32_t up = ~neg & 0xFFu;
+  if (!clear) {
+    up = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) up |= (sum_is_nonneg(x[i], c[i], y[i], minus ? -s[i] : s[i]) ? 1u : 0u) << i;
+  }
+  return up;
+}
+
+__device__ __forceinline__ uint32_t plain_byte(const float (&x)[8]) {
+  uint32_t up = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) up |= (x[i] >= 0.f ? 1u : 0u) << i;
+  return up;
+}
+
+// Both sign bytes of a lane's 16 dims.
+template <typename T, bool kHalf>
+__device__ __forceinline__ void turn16(const Run8<T>& r0, const Run8<T>& r1, const float (&c)[8], const float (&s)[8],
+                                       bool turned, uint32_t& b0, uint32_t& b1) {
+  float x[8], y[8];
+  widen8<T>(r0, x);
+  widen8<T>(r1, y);
+  if (!turned) {
+    b0 = plain_byte(x);
+    b1 = plain_byte(y);
+  } else if (kHalf) {
+    b0 = sign_byte(x, c, y, s, true);
+    b1 = sign_byte(y, c, x, s, false);
+  } else {
+    // neighbours: members a in the even places, b in the odd ones
+    float p[8], q[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = x[2 * i];
+      q[i] = x[2 * i + 1];
+      p[i + 4] = y[2 * i];
+      q[i + 4] = y[2 * i + 1];
+    }
+    uint32_t u = sign_byte(p, c, q, s, true), w = sign_byte(q, c, p, s, false);
+    // bit i of u to bit 2i, of w to bit 2i + 1
+    u = (u | (u << 4)) & 0x0F0Fu;
+    u = (u | (u << 2)) & 0x3333u;
+    u = (u | (u << 1)) & 0x5555u;
+    w = (w | (w << 4)) & 0x0F0Fu;
+    w = (w | (w << 2)) & 0x3333u;
+    w = (w | (w << 1)) & 0x5555u;
+    const uint32_t both = u | (w << 1);
+    b0 = both & 0xFFu;
+    b1 = both >> 8;
+  }
+}
+
+// Warp `wid` takes token wid / parts and the row units [part * per, (part + 1) * per) of
+// its n_heads query heads and n_kv_heads (K, V) pairs.
+template <int D, typename T, bool kHalf>
+__global__ void __launch_bounds__(32 * kWarpsPerBlock, 3) rope_write_vec_kernel(Args a, int parts, int per) {
+  constexpr int W = D / 32;
+  constexpr int G = D / 16;  // lanes a row
+  constexpr int R = 32 / G;  // rows a warp
+  constexpr int U = kUnroll<T>;
+  __shared__ __align__(16) uint8_t s_bytes[kWarpsPerBlock][U * R][D / 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int j = lane % G, g = lane / G;
+  const long long wid = (long long)blockIdx.x * kWarpsPerBlock + warp;
+  const int tok = (int)(wid / parts);
+  const int part = (int)(wid - (long long)tok * parts);
+  if (tok >= a.n_tokens) return;
+  const int b = __ldg(a.seq_ids + tok);
+  const int pos = __ldg(a.positions + tok);
+  if (b < 0 || pos < 0 || (a.rot > 0 && pos >= a.n_positions)) {
+    if (lane == 0) raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
+    return;
+  }
+  // Runs of this lane in a row, in units of 8 dims.
+  const int turning = a.rot / 16;  // lanes whose dims turn
+  const bool turned = j < turning;
+  int c0 = 2 * j, c1 = 2 * j + 1;
+  if (kHalf && turned) {
+    c0 = j;
+    c1 = turning + j;
+  }
+  float c[8], s[8];
+  if (turned) {
+    const float4* cs = reinterpret_cast<const float4*>(a.table + (long long)pos * a.rot) + 2 * j;
+    const float4* sn = reinterpret_cast<const float4*>(a.table + (long long)pos * a.rot + a.rot / 2) + 2 * j;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 p = __ldg(cs + i), q = __ldg(sn + i);
+      c[4 * i] = p.x, c[4 * i + 1] = p.y, c[4 * i + 2] = p.z, c[4 * i + 3] = p.w;
+      s[4 * i] = q.x, s[4 * i + 1] = q.y, s[4 * i + 2] = q.z, s[4 * i + 3] = q.w;
+    }
+  }
+  uint8_t(*buf)[D / 8] = s_bytes[warp];
+
+  const int u0 = part * per, u1 = min(u0 + per, a.n_heads + a.n_kv_heads);
+  const int q1 = min(u1, a.n_heads);
+  const T* q = static_cast<const T*>(a.q) + tok * a.q_ts;
+  for (int base = u0; base < q1; base += U * R) {
+    Run8<T> r[U][2];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = min(base + i * R + g, q1 - 1);  // rows beyond the last are not stored
+      r[i][0] = load8<T>(q + h * a.q_hs + 8 * c0);
+      r[i][1] = load8<T>(q + h * a.q_hs + 8 * c1);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      uint32_t b0, b1;
+      turn16<T, kHalf>(r[i][0], r[i][1], c, s, turned, b0, b1);
+      buf[i * R + g][c0] = (uint8_t)b0;
+      buf[i * R + g][c1] = (uint8_t)b1;
+    }
+    __syncwarp();
+    // The U * R rows in pieces of 16 bytes.
+    constexpr int kPieces = U * R * (D / 128);
+    if (lane < kPieces) {
+      const int row = lane / (D / 128), piece = lane % (D / 128);
+      const int h = base + row;
+      if (h < q1) {
+        const long long out = q_row_of(a, tok, b, pos, h);
+        if (out < 0) {
+          raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
+        } else {
+          *reinterpret_cast<uint4*>(a.q_words + out * W + 4 * piece) = *reinterpret_cast<const uint4*>(&buf[row][16 * piece]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  for (int base = max(u0, a.n_heads); base < u1; base += R) {
+    const int h = min(base + g, u1 - 1) - a.n_heads;
+    const T* kr = static_cast<const T*>(a.k) + tok * a.k_ts + h * a.k_hs;
+    const T* vr = static_cast<const T*>(a.v) + tok * a.v_ts + h * a.v_hs + 16 * j;
+    const Run8<T> k0 = load8<T>(kr + 8 * c0), k1 = load8<T>(kr + 8 * c1);
+    const Run8<T> v0 = load8<T>(vr), v1 = load8<T>(vr + 8);
+    const long long kv = (long long)b * a.n_kv_heads + h;
+    int slot = 0;
+    const long long out = base + g < u1 ? kv_row_of(a, tok, pos, h, kv, j == 0, &slot) : -1;
+    uint32_t b0, b1;
+    turn16<T, kHalf>(k0, k1, c, s, turned, b0, b1);
+    buf[g][c0] = (uint8_t)b0;
+    buf[g][c1] = (uint8_t)b1;
+    __syncwarp();
+    if (out >= 0) {
+      if (j < D / 128)
+        *reinterpret_cast<uint4*>(a.k_cache + out * W + 4 * j) = *reinterpret_cast<const uint4*>(&buf[g][16 * j]);
+      if (j == 0 && a.slot_positions) a.slot_positions[kv * a.pages.capacity() + slot] = pos;
+      const float scale = v_scale_of(a, kv, out);
+      float x[8], y[8];
+      widen8<T>(v0, x);
+      widen8<T>(v1, y);
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i / 4] |= v_code(x[i], scale) << (8 * (i % 4));
+        w[2 + i / 4] |= v_code(y[i], scale) << (8 * (i % 4));
+      }
+      *reinterpret_cast<uint4*>(a.v_cache + out * D + 16 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The scalar kernel: any even rotary_dim, any alignment and stride.  One warp per (token,
+// query head) and per (token, KV head); lane l takes dims l, l + 32, ..., so a ballot is
+// one sign word.
+// ---------------------------------------------------------------------------
 template <int D, typename T>
 __global__ void __launch_bounds__(32 * kWarpsPerBlock) rope_write_kernel(Args a) {
   constexpr int W = D / 32;
@@ -77,32 +326,19 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) rope_write_kernel(Args a)
   const int h = is_q ? hh : hh - a.n_heads;
   const T* row = is_q ? static_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs
                       : static_cast<const T*>(a.k) + tok * a.k_ts + h * a.k_hs;
-  long long out_row, kv = 0;
+  const long long kv = (long long)b * a.n_kv_heads + h;
+  long long out_row;
   if (is_q) {
-    const int qi = a.q_idx ? __ldg(a.q_idx + tok) : (a.seq_q == 1 ? 0 : pos);
-    out_row = ((long long)b * a.n_heads + h) * a.seq_q + qi;
-    if (qi < 0 || qi >= a.seq_q || out_row >= a.q_rows) {
+    out_row = q_row_of(a, tok, b, pos, h);
+    if (out_row < 0) {
       if (lane == 0) raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
       return;
     }
   } else {
-    kv = (long long)b * a.n_kv_heads + h;
-    const int t = a.slots ? __ldg(a.slots + (a.slots_per_head ? (long long)tok * a.n_kv_heads + h : (long long)tok)) : pos;
-    const long long cap = (long long)a.num_blocks * a.block_size;
-    if (t < 0 || (long long)t >= cap || (a.block_tables && kv >= a.bt_rows) ||
-        (a.slot_positions && kv >= a.slot_rows)) {
-      if (lane == 0) raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
-      return;
-    }
-    const int page = t / a.block_size;
-    const long long id =
-        a.block_tables ? (long long)__ldg(a.block_tables + kv * a.num_blocks + page) : kv * a.num_blocks + page;
-    if (id < 0 || id >= a.pool_rows / a.block_size) {
-      if (lane == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
-      return;
-    }
-    out_row = id * a.block_size + (t - page * a.block_size);
-    if (a.slot_positions && lane == 0) a.slot_positions[kv * cap + t] = pos;
+    int slot;
+    out_row = kv_row_of(a, tok, pos, h, kv, lane == 0, &slot);
+    if (out_row < 0) return;
+    if (a.slot_positions && lane == 0) a.slot_positions[kv * a.pages.capacity() + slot] = pos;
   }
   const int half = a.rot / 2;
   const float* cs = a.table + (long long)pos * a.rot;
@@ -127,33 +363,50 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) rope_write_kernel(Args a)
   }
   if (lane < W) (is_q ? a.q_words : a.k_cache)[out_row * W + lane] = word;
   if (is_q) return;
-  const long long si = a.v_scale_numel == 1 ? 0 : (a.v_scale_numel == a.pool_rows ? out_row : kv % a.v_scale_numel);
-  const float scale = __ldg(a.v_scale + si);
+  const float scale = v_scale_of(a, kv, out_row);
   const T* vr = static_cast<const T*>(a.v) + tok * a.v_ts + h * a.v_hs;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    float y = __fdiv_rn(kvw::to_f32<T>(vr[32 * w + lane]), scale);
-    if (y == y) y = fminf(fmaxf(y, -448.f), 448.f);
-    a.v_cache[out_row * D + 32 * w + lane] = (uint8_t)kvw::e4m3_code(y);
-  }
+  for (int w = 0; w < W; ++w)
+    a.v_cache[out_row * D + 32 * w + lane] = (uint8_t)v_code(kvw::to_f32<T>(vr[32 * w + lane]), scale);
 }
 
-template <int D>
-inline cudaError_t launch_d(const Args& a, int in_dtype, cudaStream_t st) {
-  const long long warps = (long long)a.n_tokens * (a.n_heads + a.n_kv_heads);
-  const unsigned grid = (unsigned)((warps + kWarpsPerBlock - 1) / kWarpsPerBlock);
-  if (in_dtype == HYPERION_DTYPE_F32) {
-    rope_write_kernel<D, float><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a);
-  } else if (in_dtype == HYPERION_DTYPE_BF16) {
-    rope_write_kernel<D, __nv_bfloat16><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a);
+inline bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <int D, typename T>
+inline cudaError_t launch_t(const Args& a, int n_sm, cudaStream_t st) {
+  constexpr long long kPer16 = 16 / sizeof(T);
+  const long long units = a.n_heads + a.n_kv_heads;
+  const bool vec = a.rot % 16 == 0 && on16(a.table) && on16(a.q) && on16(a.k) && on16(a.v) &&
+                   (a.q_ts | a.q_hs | a.k_ts | a.k_hs | a.v_ts | a.v_hs) % kPer16 == 0;
+  if (vec) {
+    // Enough warps to fill the device, no more than one round of rows each.
+    constexpr int R = 512 / D;
+    const long long want = (32LL * n_sm + a.n_tokens - 1) / a.n_tokens;
+    const long long parts0 = std::max(1LL, std::min(want, (units + R - 1) / R));
+    const int per = (int)((((units + parts0 - 1) / parts0) + R - 1) / R * R);
+    const int parts = (int)((units + per - 1) / per);
+    const unsigned grid = (unsigned)(((long long)a.n_tokens * parts + kWarpsPerBlock - 1) / kWarpsPerBlock);
+    if (a.interleaved) {
+      rope_write_vec_kernel<D, T, false><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a, parts, per);
+    } else {
+      rope_write_vec_kernel<D, T, true><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a, parts, per);
+    }
   } else {
-    rope_write_kernel<D, __half><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a);
+    const unsigned grid = (unsigned)((a.n_tokens * units + kWarpsPerBlock - 1) / kWarpsPerBlock);
+    rope_write_kernel<D, T><<<grid, 32 * kWarpsPerBlock, 0, st>>>(a);
   }
   return cudaGetLastError();
 }
 
-inline cudaError_t launch(const Args& a, int head_dim, int in_dtype, cudaStream_t st) {
-  return head_dim == 256 ? launch_d<256>(a, in_dtype, st) : launch_d<128>(a, in_dtype, st);
+template <int D>
+inline cudaError_t launch_d(const Args& a, int in_dtype, int n_sm, cudaStream_t st) {
+  if (in_dtype == HYPERION_DTYPE_F32) return launch_t<D, float>(a, n_sm, st);
+  if (in_dtype == HYPERION_DTYPE_BF16) return launch_t<D, __nv_bfloat16>(a, n_sm, st);
+  return launch_t<D, __half>(a, n_sm, st);
+}
+
+inline cudaError_t launch(const Args& a, int head_dim, int in_dtype, int n_sm, cudaStream_t st) {
+  return head_dim == 256 ? launch_d<256>(a, in_dtype, n_sm, st) : launch_d<128>(a, in_dtype, n_sm, st);
 }
 
 }  // namespace rope

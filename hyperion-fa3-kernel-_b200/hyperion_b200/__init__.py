@@ -65,6 +65,11 @@ _captured: set = set()  # keys of workspaces that a captured graph may hold the 
 _retired: list = []  # outgrown workspaces of those keys: a graph replays on them
 
 
+def _raw_stream(idx: int) -> int:
+    """cudaStream_t of the current stream of device idx, without the Stream object around it (2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(idx)
+
+
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Workspace (work counter, error word, split-KV partials) of the current stream of
     `device`, grown on demand.
@@ -77,7 +82,7 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     the graph goes on using its address."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     dev = torch.device("cuda", idx)
-    key = (idx, torch.cuda.current_stream(dev).cuda_stream)
+    key = (idx, _raw_stream(idx))
     with _ws_lock:
         ws = _workspaces.get(key)
         capturing = torch.cuda.is_current_stream_capturing()

@@ -20,42 +20,50 @@ import ctypes
 
 import torch
 
-from . import _capi, _nbytes, _workspace
+from . import _capi, _nbytes, _raw_stream, _workspace
 
 _IN_DTYPES = {torch.float16: _capi.DTYPE_F16, torch.bfloat16: _capi.DTYPE_BF16, torch.float32: _capi.DTYPE_F32}
 _LAYOUTS = {"half": _capi.ROPE_HALF, "interleaved": _capi.ROPE_INTERLEAVED}
 _WS_BYTES = 1 << 16
+_INT_MAX = 0x7FFFFFFF
 
 
-def _check(cond: bool, name: str, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(f"{name}: {msg}")
+def _refuse(name: str, msg: str) -> None:
+    raise RuntimeError(f"{name}: {msg}")
 
 
-def _check_device(name: str, dev: torch.device, **tensors) -> None:
-    _check(dev.type == "cuda", name, "the caches must be CUDA tensors")
-    for arg, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{name}: {arg} must be on {dev}")
-
-
-def _check_contiguous(name: str, **tensors) -> None:
-    for arg, t in tensors.items():
-        if t is not None and not t.is_contiguous():
-            raise RuntimeError(f"{name}: {arg} must be contiguous")
+def _check_tensors(name: str, dev: torch.device, names: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor given is contiguous and on the caches' device."""
+    idx = dev.index
+    for t in tensors:
+        if t is not None and not (t.is_contiguous() and t.get_device() == idx):
+            break
+    else:
+        return
+    named = [(n, t) for n, t in zip(names.split(), tensors) if t is not None]
+    for n, t in named:
+        if not t.is_contiguous():
+            _refuse(name, f"{n} must be contiguous")
+    if dev.type != "cuda":
+        _refuse(name, "the caches must be CUDA tensors")
+    for n, t in named:
+        if t.device != dev:
+            _refuse(name, f"{n} must be on {dev}")
 
 
 def _tables(name: str, block_tables: Optional[torch.Tensor]):
     """(address, numel) of the block tables; (None, 0) for the contiguous layout."""
     if block_tables is None or block_tables.numel() == 0:
         return None, 0
-    _check(block_tables.dtype == torch.int32, name, "block_tables must be int32")
+    if not (block_tables.dtype == torch.int32):
+        _refuse(name, "block_tables must be int32")
     return block_tables.data_ptr(), block_tables.numel()
 
 
 def _same_or_apart(name: str, arg: str, a: torch.Tensor, b: torch.Tensor) -> None:
     p, q = a.data_ptr(), b.data_ptr()
-    _check(p == q or p + _nbytes(a) <= q or q + _nbytes(b) <= p, name, f"{arg} overlaps its input")
+    if not (p == q or p + _nbytes(a) <= q or q + _nbytes(b) <= p):
+        _refuse(name, f"{arg} overlaps its input")
 
 
 def _call(name: str, fn, args, dev: torch.device, scratch: int = 0) -> None:
@@ -67,7 +75,7 @@ def _call(name: str, fn, args, dev: torch.device, scratch: int = 0) -> None:
         buf = torch.empty(scratch, dtype=torch.uint8, device=dev)
         args.scratch, args.scratch_bytes = buf.data_ptr(), scratch
     ws = _workspace(dev, _WS_BYTES)
-    rc = fn(ctypes.byref(args), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+    rc = fn(ctypes.byref(args), ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
     if rc != _capi.HYPERION_OK:
         raise RuntimeError(f"{name} failed (status {rc}): {_capi.last_error()}")
 
@@ -101,55 +109,66 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
     positions and pages out of range are skipped and flagged.  Two tokens of a call must
     not name the same slot or query row."""
     name = "rope_cache_write"
-    _check(Q_new.dtype in _IN_DTYPES and K_new.dtype == Q_new.dtype and V_new.dtype == Q_new.dtype, name,
-           "Q_new, K_new and V_new must share a float16, bfloat16 or float32 dtype")
-    _check(Q_new.dim() == 3 and K_new.dim() == 3 and V_new.shape == K_new.shape, name,
-           "Q_new must be [n_tokens, n_heads, head_dim], K_new and V_new [n_tokens, n_kv_heads, head_dim]")
+    if not (Q_new.dtype in _IN_DTYPES and K_new.dtype == Q_new.dtype and V_new.dtype == Q_new.dtype):
+        _refuse(name, "Q_new, K_new and V_new must share a float16, bfloat16 or float32 dtype")
+    if not (Q_new.dim() == 3 and K_new.dim() == 3 and V_new.shape == K_new.shape):
+        _refuse(name, "Q_new must be [n_tokens, n_heads, head_dim], K_new and V_new [n_tokens, n_kv_heads, head_dim]")
     n_tokens, n_heads, head_dim = Q_new.shape
     n_kv = K_new.shape[1]
-    _check(K_new.shape[0] == n_tokens and K_new.shape[2] == head_dim, name, "Q_new and K_new differ in tokens or head_dim")
-    _check(head_dim in (128, 256), name, "head_dim must be 128 or 256")
-    _check(n_heads >= 1 and n_kv >= 1, name, "n_heads and n_kv_heads must be >= 1")
+    if not (K_new.shape[0] == n_tokens and K_new.shape[2] == head_dim):
+        _refuse(name, "Q_new and K_new differ in tokens or head_dim")
+    if not (head_dim in (128, 256)):
+        _refuse(name, "head_dim must be 128 or 256")
+    if not (n_heads >= 1 and n_kv >= 1):
+        _refuse(name, "n_heads and n_kv_heads must be >= 1")
     qs, ks, vs = Q_new.stride(), K_new.stride(), V_new.stride()
-    _check(n_tokens == 0 or (qs[2] == 1 and ks[2] == 1 and vs[2] == 1), name, "the dims of a head must be contiguous")
-    _check(seq_ids.dtype == torch.int32 and positions.dtype == torch.int32 and seq_ids.numel() == n_tokens
-           and positions.numel() == n_tokens, name, "seq_ids and positions must be int32 [n_tokens]")
-    _check(q_idx is None or (q_idx.dtype == torch.int32 and q_idx.numel() == n_tokens), name,
-           "q_idx must be int32 [n_tokens]")
+    if not (n_tokens == 0 or (qs[2] == 1 and ks[2] == 1 and vs[2] == 1)):
+        _refuse(name, "the dims of a head must be contiguous")
+    if not (seq_ids.dtype == torch.int32 and positions.dtype == torch.int32 and seq_ids.numel() == n_tokens
+            and positions.numel() == n_tokens):
+        _refuse(name, "seq_ids and positions must be int32 [n_tokens]")
+    if not (q_idx is None or (q_idx.dtype == torch.int32 and q_idx.numel() == n_tokens)):
+        _refuse(name, "q_idx must be int32 [n_tokens]")
     per_head = 0
     if slots is not None:
         per_head = 1 if slots.dim() == 2 else 0
-        _check(slots.dtype == torch.int32 and tuple(slots.shape) == ((n_tokens, n_kv) if per_head else (n_tokens,)), name,
-               "slots must be int32 [n_tokens] or [n_tokens, n_kv_heads]")
+        if not (slots.dtype == torch.int32 and tuple(slots.shape) == ((n_tokens, n_kv) if per_head else (n_tokens,))):
+            _refuse(name, "slots must be int32 [n_tokens] or [n_tokens, n_kv_heads]")
     rot = n_pos = 0
     if rope is not None:
-        _check(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[1] == 2 and rope.shape[0] >= 1, name,
-               "rope must be float32 [n_positions, 2, rotary_dim / 2]")
+        if not (rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[1] == 2 and rope.shape[0] >= 1):
+            _refuse(name, "rope must be float32 [n_positions, 2, rotary_dim / 2]")
         n_pos, rot = rope.shape[0], 2 * rope.shape[2]
-        _check(rot <= head_dim, name, "rope turns more dims than head_dim")
-    _check(layout in _LAYOUTS, name, "layout must be 'half' or 'interleaved'")
-    _check(seq_q >= 1, name, "seq_q must be >= 1")
-    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
-    _check(V_scale.dtype == torch.float32 and V_scale.numel() >= 1, name, "V_scale must be a non-empty float32 tensor")
-    _check(V_cache.element_size() == 1 and V_cache.numel() % head_dim == 0 and V_cache.numel() > 0, name,
-           "V_cache must hold one byte per element, [pool_rows, head_dim]")
+        if not (rot <= head_dim):
+            _refuse(name, "rope turns more dims than head_dim")
+    if not (layout in _LAYOUTS):
+        _refuse(name, "layout must be 'half' or 'interleaved'")
+    if not (1 <= seq_q <= _INT_MAX):
+        _refuse(name, "seq_q must be >= 1 and fit int32")
+    if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
+        _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
+    if not (V_scale.dtype == torch.float32 and V_scale.numel() >= 1):
+        _refuse(name, "V_scale must be a non-empty float32 tensor")
+    if not (V_cache.element_size() == 1 and V_cache.numel() % head_dim == 0 and V_cache.numel() > 0):
+        _refuse(name, "V_cache must hold one byte per element, [pool_rows, head_dim]")
     pool_rows = V_cache.numel() // head_dim
-    _check(_nbytes(K_cache) >= pool_rows * head_dim // 8, name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
-    _check(_nbytes(Q_words) % (head_dim // 8) == 0, name, "Q_words bytes must be a multiple of head_dim/8")
+    if not (_nbytes(K_cache) >= pool_rows * head_dim // 8):
+        _refuse(name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
+    if not (_nbytes(Q_words) % (head_dim // 8) == 0):
+        _refuse(name, "Q_words bytes must be a multiple of head_dim/8")
     slot_rows = 0
     if slot_positions is not None:
-        _check(slot_positions.dtype == torch.int32 and slot_positions.dim() == 2
-               and slot_positions.shape[1] == block_size * num_blocks, name,
-               "slot_positions must be int32 [cache rows, num_blocks * block_size]")
+        if not (slot_positions.dtype == torch.int32 and slot_positions.dim() == 2
+                and slot_positions.shape[1] == block_size * num_blocks):
+            _refuse(name, "slot_positions must be int32 [cache rows, num_blocks * block_size]")
         slot_rows = slot_positions.shape[0]
     bt, bt_numel = _tables(name, block_tables)
-    _check_contiguous(name, seq_ids=seq_ids, positions=positions, rope=rope, block_tables=block_tables, V_scale=V_scale,
-                      Q_words=Q_words, K_cache=K_cache, V_cache=V_cache, q_idx=q_idx, slots=slots,
-                      slot_positions=slot_positions)
     dev = K_cache.device
-    _check_device(name, dev, Q_new=Q_new, K_new=K_new, V_new=V_new, seq_ids=seq_ids, positions=positions, rope=rope,
-                  block_tables=block_tables, V_scale=V_scale, Q_words=Q_words, V_cache=V_cache, q_idx=q_idx, slots=slots,
-                  slot_positions=slot_positions)
+    _check_tensors(name, dev, "seq_ids positions rope block_tables V_scale Q_words K_cache V_cache q_idx slots slot_positions",
+                   seq_ids, positions, rope, block_tables, V_scale, Q_words, K_cache, V_cache, q_idx, slots, slot_positions)
+    for t in (Q_new, K_new, V_new):
+        if t.device != dev:
+            _refuse(name, f"Q_new, K_new and V_new must be on {dev}")
     args = _capi.RopeWriteArgs(
         Q_new.data_ptr(), K_new.data_ptr(), V_new.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
         _IN_DTYPES[Q_new.dtype], n_tokens, n_heads, n_kv, head_dim, rot, _LAYOUTS[layout], n_pos,
@@ -181,32 +200,37 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
     weights: float32 [cache rows, >= num_blocks * block_size]; out: as weights, weights
     itself by default.  Returns out.  The same inputs give the same bits."""
     name = "accumulate_key_weights"
-    _check(head_dim in (128, 256), name, "head_dim must be 128 or 256")
-    _check(context_lens.dtype == torch.int32, name, "context_lens must be int32")
+    if not (head_dim in (128, 256)):
+        _refuse(name, "head_dim must be 128 or 256")
+    if not (context_lens.dtype == torch.int32):
+        _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
     n_q = seq_q if n_q is None else n_q
-    _check(kv_group >= 1 and seq_q >= 1 and n_q >= 1, name, "kv_group, seq_q and n_q must be >= 1")
-    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
+    if not (1 <= kv_group <= _INT_MAX and 1 <= seq_q <= _INT_MAX and 1 <= n_q <= _INT_MAX):
+        _refuse(name, "kv_group, seq_q and n_q must be >= 1 and fit int32")
+    if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
+        _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
     row_bytes = head_dim // 8
-    _check(_nbytes(Q) >= n_kv * kv_group * seq_q * row_bytes, name, "Q smaller than its rows of head_dim/8 bytes")
-    _check(_nbytes(K_cache) % row_bytes == 0 and K_cache.numel() > 0, name, "K_cache must be [pool_rows, head_dim/32] words")
+    if not (_nbytes(Q) >= n_kv * kv_group * seq_q * row_bytes):
+        _refuse(name, "Q smaller than its rows of head_dim/8 bytes")
+    if not (_nbytes(K_cache) % row_bytes == 0 and K_cache.numel() > 0):
+        _refuse(name, "K_cache must be [pool_rows, head_dim/32] words")
     out = weights if out is None else out
     for arg, t in (("weights", weights), ("out", out)):
-        _check(t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == n_kv
-               and t.shape[1] >= block_size * num_blocks, name,
-               f"{arg} must be float32 [cache rows, >= num_blocks * block_size]")
-    _check(out.shape == weights.shape, name, "out must have the shape of weights")
-    _check(q_first is None or (q_first.dtype == torch.int32 and q_first.numel() == n_kv), name,
-           "q_first must be int32 [cache rows]")
+        if not (t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks):
+            _refuse(name, f"{arg} must be float32 [cache rows, >= num_blocks * block_size]")
+    if not (out.shape == weights.shape):
+        _refuse(name, "out must have the shape of weights")
+    if not (q_first is None or (q_first.dtype == torch.int32 and q_first.numel() == n_kv)):
+        _refuse(name, "q_first must be int32 [cache rows]")
     bt, bt_numel = _tables(name, block_tables)
-    _check(bt_numel == 0 or bt_numel >= n_kv * num_blocks, name, "block_tables numel < cache rows * num_blocks")
-    _check_contiguous(name, Q=Q, K_cache=K_cache, context_lens=context_lens, block_tables=block_tables, weights=weights,
-                      out=out, q_first=q_first)
+    if not (bt_numel == 0 or bt_numel >= n_kv * num_blocks):
+        _refuse(name, "block_tables numel < cache rows * num_blocks")
+    dev = K_cache.device
     if out is not weights:
         _same_or_apart(name, "out", weights, out)
-    dev = K_cache.device
-    _check_device(name, dev, Q=Q, context_lens=context_lens, block_tables=block_tables, weights=weights, out=out,
-                  q_first=q_first)
+    _check_tensors(name, dev, "Q K_cache context_lens block_tables weights out q_first",
+                   Q, K_cache, context_lens, block_tables, weights, out, q_first)
     if n_kv == 0:
         return out
     args = _capi.KeyWeightsArgs(
@@ -242,44 +266,49 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     The new lengths, weights and positions go to the *_out tensors, by default the inputs
     themselves.  Returns the new lengths (context_lens_out).  Rows must not share pages."""
     name = "evict_keys"
-    _check(V_cache.element_size() == 1 and V_cache.dim() == 2 and V_cache.shape[1] in (128, 256) and V_cache.shape[0] > 0,
-           name, "V_cache must hold one byte per element, [pool_rows, head_dim] with head_dim 128 or 256")
+    if not (V_cache.element_size() == 1 and V_cache.dim() == 2 and V_cache.shape[1] in (128, 256) and V_cache.shape[0] > 0):
+        _refuse(name, "V_cache must hold one byte per element, [pool_rows, head_dim] with head_dim 128 or 256")
     pool_rows, head_dim = V_cache.shape
-    _check(_nbytes(K_cache) >= pool_rows * head_dim // 8, name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
-    _check(context_lens.dtype == torch.int32, name, "context_lens must be int32")
+    if not (_nbytes(K_cache) >= pool_rows * head_dim // 8):
+        _refuse(name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
+    if not (context_lens.dtype == torch.int32):
+        _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
-    _check(block_size >= 1 and num_blocks >= 1, name, "block_size and num_blocks must be >= 1")
+    if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
+        _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
     ctx_out = context_lens if context_lens_out is None else context_lens_out
     w_out = weights if weights_out is None else weights_out
     p_out = positions if positions_out is None else positions_out
-    _check(ctx_out.dtype == torch.int32 and ctx_out.numel() == n_kv, name, "context_lens_out must be int32 [cache rows]")
+    if not (ctx_out.dtype == torch.int32 and ctx_out.numel() == n_kv):
+        _refuse(name, "context_lens_out must be int32 [cache rows]")
     for arg, t, dt in (("weights", weights, torch.float32), ("weights_out", w_out, torch.float32),
                        ("positions", positions, torch.int32), ("positions_out", p_out, torch.int32)):
-        _check(t.dtype == dt and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks
-               and t.shape == weights.shape, name,
-               f"{arg} must be {str(dt)[6:]} [cache rows, >= num_blocks * block_size], all four of one shape")
+        if not (t.dtype == dt and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks
+                and t.shape == weights.shape):
+            _refuse(name, f"{arg} must be {str(dt)[6:]} [cache rows, >= num_blocks * block_size], all four of one shape")
     keep_rows = keep if isinstance(keep, torch.Tensor) else None
     if keep_rows is not None:
-        _check(keep.dtype == torch.int32 and keep.numel() == n_kv, name, "keep must be an int or int32 [cache rows]")
+        if not (keep.dtype == torch.int32 and keep.numel() == n_kv):
+            _refuse(name, "keep must be an int or int32 [cache rows]")
     else:
-        _check(keep >= 0, name, "keep must be >= 0")
-        keep = min(keep, 0x7FFFFFFF)
-    _check(0 <= sink <= 0x7FFFFFFF and 0 <= recent <= 0x7FFFFFFF, name, "sink and recent must be >= 0 and fit int32")
-    _check(V_scale is None or (V_scale.dtype == torch.float32 and V_scale.numel() == pool_rows), name,
-           "V_scale must be float32 [pool_rows], one scale per slot; other scales do not move")
+        if not (keep >= 0):
+            _refuse(name, "keep must be >= 0")
+        keep = min(keep, _INT_MAX)
+    if not (0 <= sink <= _INT_MAX and 0 <= recent <= _INT_MAX):
+        _refuse(name, "sink and recent must be >= 0 and fit int32")
+    if not (V_scale is None or (V_scale.dtype == torch.float32 and V_scale.numel() == pool_rows)):
+        _refuse(name, "V_scale must be float32 [pool_rows], one scale per slot; other scales do not move")
     bt, bt_numel = _tables(name, block_tables)
-    _check(bt_numel == 0 or bt_numel >= n_kv * num_blocks, name, "block_tables numel < cache rows * num_blocks")
-    _check_contiguous(name, K_cache=K_cache, V_cache=V_cache, context_lens=context_lens, block_tables=block_tables,
-                      weights=weights, positions=positions, keep=keep_rows, V_scale=V_scale, context_lens_out=ctx_out,
-                      weights_out=w_out, positions_out=p_out)
+    if not (bt_numel == 0 or bt_numel >= n_kv * num_blocks):
+        _refuse(name, "block_tables numel < cache rows * num_blocks")
     for arg, a, b in (("context_lens_out", context_lens, ctx_out), ("weights_out", weights, w_out),
                       ("positions_out", positions, p_out)):
         if a is not b:
             _same_or_apart(name, arg, a, b)
     dev = K_cache.device
-    _check_device(name, dev, V_cache=V_cache, context_lens=context_lens, block_tables=block_tables, weights=weights,
-                  positions=positions, keep=keep_rows, V_scale=V_scale, context_lens_out=ctx_out, weights_out=w_out,
-                  positions_out=p_out)
+    _check_tensors(name, dev, "K_cache V_cache context_lens block_tables weights positions keep V_scale context_lens_out "
+                   "weights_out positions_out", K_cache, V_cache, context_lens, block_tables, weights, positions, keep_rows,
+                   V_scale, ctx_out, w_out, p_out)
     if n_kv == 0:
         return ctx_out
     args = _capi.EvictArgs(

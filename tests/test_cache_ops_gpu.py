@@ -319,6 +319,23 @@ def test_weights_whole_causal_prompt_and_windows_past_the_rows(hyperion):
     _weights_check(hyperion, c, causal=True, first=np.array([-2147483648, 2147483647, 0], np.int32), n_q=3)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("group, n_q", [(1, 2), (2, 5), (4, 4)])
+def test_weights_short_windows_partly_outside_the_rows(hyperion, group, n_q, causal):
+    c = _weights_case([33, 2500, 40, 900], 1, group, seq_q=50, seed=n_q)
+    for first in ([-1, 48, 0, 20], [-100, 50, -n_q, 49]):
+        _weights_check(hyperion, c, causal=causal, first=np.array(first, np.int32), n_q=n_q)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+def test_weights_many_rows_of_short_and_long_contexts(hyperion, D):
+    """Enough keys for the blocks of many keys a thread, ends inside and between them."""
+    _weights_check(hyperion, _weights_case([2048, 2047, 2049, 1, 0, 4096, 100, 3000] * 20, 1, 4, D, block=16, nb=256, seed=D))
+    c = _weights_case([4100] * 8 + [17] * 150, 1, 3, D, block=1000, seed=D)
+    c["table"][3, 2], c["table"][5, 0] = -1, 1 << 29
+    _weights_check(hyperion, c, err=hyperion.DEVERR_BAD_BLOCK)
+
+
 @pytest.mark.parametrize("inv", [-0.09, 0.0, 1.0, -3.0, 1e4])
 @pytest.mark.parametrize("seq_q", [1, 40])
 def test_weights_scales_of_either_sign_and_beyond_the_clamp(hyperion, inv, seq_q):

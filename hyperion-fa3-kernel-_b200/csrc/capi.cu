@@ -127,6 +127,8 @@ int get_dev(const DevInfo** out) {
       di.tile_why = why;
       cudaGetLastError();
     }
+    e = hyp::evict::setup();
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(eviction)");
     di.mma_ok = hyp::rmma::setup(di.mma_ctas, di.mma_smem) == cudaSuccess && di.mma_ctas > 0;
     if (!di.mma_ok) {
       di.mma_ctas = 0;
@@ -787,7 +789,7 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
 
 extern "C" size_t hyperion_evict_scratch_bytes(int32_t n_kv, int32_t block_size, int32_t num_blocks) {
   if (n_kv < 1 || block_size < 1 || num_blocks < 1) return 0;
-  return hyp::evict::scratch_bytes(n_kv, block_size, num_blocks);
+  return hyp::evict::scratch_bytes(n_kv, (long long)block_size * num_blocks);
 }
 
 extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace, size_t workspace_bytes,
@@ -809,6 +811,8 @@ extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace
     return fail(HYPERION_ERR_INVALID_ARG, "a tensor pointer is NULL");
   if (!aligned(x->k_cache, 16) || !aligned(x->v_cache, 16))
     return fail(HYPERION_ERR_INVALID_ARG, "k_cache and v_cache must be 16-byte aligned");
+  if (!aligned(x->weights, 4) || !aligned(x->weights_out, 4) || !aligned(x->positions, 4) || !aligned(x->positions_out, 4))
+    return fail(HYPERION_ERR_INVALID_ARG, "weights and positions must be aligned to their element size");
   const size_t need = hyperion_evict_scratch_bytes(x->n_kv, x->block_size, x->num_blocks);
   if (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16))
     return fail(HYPERION_ERR_WORKSPACE,
@@ -831,9 +835,12 @@ extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace
   a.keep = x->keep;
   a.sink = x->sink;
   a.recent = x->recent;
-  a.holes = static_cast<int32_t*>(x->scratch);
-  a.hole_ld = hyp::evict::hole_ld(x->block_size, x->num_blocks);
+  a.lists = static_cast<int32_t*>(x->scratch);
+  a.list_ld = hyp::evict::list_ld((long long)x->block_size * x->num_blocks);
   a.err = error_word(workspace);
+  const DevInfo* di = nullptr;
+  rc = get_dev(&di);
+  if (rc) return rc;
   const cudaError_t e = hyp::evict::launch(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "eviction launch");
 }

@@ -471,7 +471,7 @@ def test_evict_page_sizes_and_row_budgets(hyperion, block, nb, D, slot_scale):
 
 
 @pytest.mark.parametrize("lens, keep", [([4097], 4096), ([4096, 5000], 2048), ([20000, 3], 777), ([70001], 35000),
-                                        ([140000], 4096), ([300000, 17], 299999)])
+                                        ([140000], 4096), ([300000, 17], 299999), ([500000, 3, 1000], 499000)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_evict_long_rows(hyperion, lens, keep, in_place):
     _evict_check(hyperion, _evict_case(lens, block=64, seed=keep), keep, 4, 100, in_place=in_place)

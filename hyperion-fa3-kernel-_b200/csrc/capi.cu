@@ -799,6 +799,7 @@ extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace
   if (x->n_kv < 0) return fail(HYPERION_ERR_INVALID_ARG, "n_kv < 0");
   if (x->keep_rows == nullptr && x->keep < 0) return fail(HYPERION_ERR_INVALID_ARG, "keep < 0");
   if (x->sink < 0 || x->recent < 0) return fail(HYPERION_ERR_INVALID_ARG, "sink and recent must be >= 0");
+  if (x->pool_rows > 0xffffffffLL) return fail(HYPERION_ERR_UNSUPPORTED, "pool_rows exceeds 32 bits");
   int rc = check_pages(x->block_tables, x->block_tables_numel, x->n_kv, x->block_size, x->num_blocks, x->pool_rows);
   if (rc) return rc;
   if (x->ld < (int64_t)x->block_size * x->num_blocks)
@@ -836,12 +837,14 @@ extern "C" int hyperion_evict_keys(const hyperion_evict_args* x, void* workspace
   a.sink = x->sink;
   a.recent = x->recent;
   a.lists = static_cast<int32_t*>(x->scratch);
-  a.list_ld = hyp::evict::list_ld((long long)x->block_size * x->num_blocks);
+  const long long cap = (long long)x->block_size * x->num_blocks;
+  a.list_ld = hyp::evict::list_ld(cap);
+  a.counts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(x->scratch) + hyp::evict::lists_bytes(x->n_kv, cap));
   a.err = error_word(workspace);
   const DevInfo* di = nullptr;
   rc = get_dev(&di);
   if (rc) return rc;
-  const cudaError_t e = hyp::evict::launch(a, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = hyp::evict::launch(a, di->n_sm, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "eviction launch");
 }
 

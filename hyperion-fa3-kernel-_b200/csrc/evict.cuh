@@ -40,6 +40,7 @@ struct Args {
   int keep, sink, recent;
   int32_t* lists;  // [n_kv, 2, list_ld]: slots that empty below m, kept slots at or beyond it
   long long list_ld;
+  int32_t* counts;  // [n_kv]: moves of each row
   uint32_t* err;
 };
 
@@ -51,31 +52,36 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 // ---------------------------------------------------------------------------
-// The kernel: a cluster of up to 16 blocks per row, each with its part of the row's ranks
-// and positions in shared memory.
+// select_kernel: a cluster of up to 16 blocks per row, each with its part of the row's
+// ranks in shared memory.
 //
 //   1. Read weights and positions once; the row's newest position and the range of its
 //      ranks by way of distributed shared memory.
 //   2. The m-th largest rank, by histograms of kBins equal intervals of the range that is
-//      left: 10 bits a turn, so 3 turns for sums of one sign, fewer when an interval is
-//      kept whole.  The blocks add their histograms up over distributed shared memory.
-//   3. Each warp walks its neighbouring slots with ballots: counts of slots that empty and
-//      of keys that move, then their places in the row's two lists (in slot order).
-//   4. The list is dealt evenly to the blocks; D / 16 lanes copy a key's codes 16 bytes each.
+//      left (10 bits a turn), until an interval is kept whole or holds at most kGather
+//      ranks: those are gathered and one warp finds the rank among them bit by bit.  Sums
+//      of attention weights take one or two turns.
+//   3. A bit per slot says what is kept.  A thread turns a word of 32 slots into its part
+//      of the row's two lists (slots that empty below m, keys that move), in slot order.
+//
+// move_kernel: the moves of all rows, 128 a block, whichever row they belong to.
 // ---------------------------------------------------------------------------
 constexpr int kBins = 1024;
+constexpr int kGather = 256;
 constexpr int kMaxCluster = 16;
-constexpr int kMovesInFlight = 4;  // keys a lane group copies at once
 
 struct Shared {
   int hist[2][kBins];
+  uint32_t cand[kGather];   // this block's ranks of the gathered interval, relative to it
+  uint32_t found[kGather];  // the row's
+  int n_cand;
   int newest, n_protected;
   uint32_t lo, hi;
-  int counts[2];  // slots that empty, keys that move
+  int counts;  // slots that empty | keys that move << 16
   // within the block
-  int warp_a[32], warp_b[32];
+  int warp_a[32];
   uint32_t warp_lo[32], warp_hi[32];
-  int pick[3];
+  int pick[4];
 };
 
 // Exclusive sum over the block's threads of x; *total its whole.  All threads call.
@@ -96,16 +102,24 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int warps, int* to
   return before + inc - x;
 }
 
-template <int NT>
-__global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys) {
+// Bits of word `at` (slots at .. at + 31) that lie below `end`.
+__device__ __forceinline__ uint32_t bits_below(int at, int end) {
+  const int k = end - at;
+  return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
+}
+
+template <int NT, int kBlocks>
+__global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster, int keys) {
   namespace cg = cooperative_groups;
   constexpr int kWarps = NT / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& sm = *reinterpret_cast<Shared*>(smem);
   uint32_t* s_rank = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));  // [keys]
-  int32_t* s_pos = reinterpret_cast<int32_t*>(s_rank + keys);             // [keys]
+  uint32_t* s_kept = s_rank + keys;                                       // [keys / 32]
+  uint32_t* s_equal = s_kept + keys / 32;                                 // [keys / 32]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / cluster, part = blockIdx.x - r * cluster;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = a.pages.context(__ldcg(a.ctx_in + r), a.err, part == 0 && tid == 0);
   const int m = min(n, max(a.keep_rows ? __ldg(a.keep_rows + r) : a.keep, 0));
   const int per = ((n + cluster - 1) / cluster + 31) & ~31;
@@ -119,7 +133,10 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
       if (w_out != w) w_out[t] = w[t];
       if (pos_out != pos) pos_out[t] = pos[t];
     }
-    if (part == 0 && tid == 0) a.ctx_out[r] = m;
+    if (part == 0 && tid == 0) {
+      a.ctx_out[r] = m;
+      a.counts[r] = 0;
+    }
     return;
   }
   auto all = cg::this_cluster();
@@ -128,17 +145,16 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
     else __syncthreads();
   };
   auto peer = [&](int p) { return cluster > 1 ? all.map_shared_rank(&sm, p) : &sm; };
+  const int other = lane < cluster ? lane : 0;  // the block whose numbers this lane looks at
 
-  // 1. Ranks, positions, newest position, range of the ranks.
+  // 1. Ranks, newest position, range of the ranks.
   int newest = INT_MIN;
   uint32_t low = 0xffffffffu, high = 0;
 #pragma unroll 4
   for (int t = tid; t < len; t += NT) {
     const uint32_t x = rank_of(w[t]);
-    const int32_t p = pos[t];
     s_rank[t] = x;
-    s_pos[t] = p;
-    newest = max(newest, p);
+    newest = max(newest, pos[t]);
     low = min(low, x);
     high = max(high, x);
   }
@@ -152,23 +168,20 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
     newest = __reduce_max_sync(0xffffffffu, lane < kWarps ? sm.warp_a[lane] : INT_MIN);
     low = __reduce_min_sync(0xffffffffu, lane < kWarps ? sm.warp_lo[lane] : 0xffffffffu);
     high = __reduce_max_sync(0xffffffffu, lane < kWarps ? sm.warp_hi[lane] : 0u);
-    if (lane == 0) sm.newest = newest, sm.lo = low, sm.hi = high, sm.n_protected = 0;
+    if (lane == 0) sm.newest = newest, sm.lo = low, sm.hi = high, sm.n_protected = 0, sm.n_cand = 0;
   }
   sync_all();
-  {
-    const bool on = lane < cluster;
-    const Shared* of = peer(on ? lane : 0);
-    newest = __reduce_max_sync(0xffffffffu, of->newest);
-    low = __reduce_min_sync(0xffffffffu, of->lo);
-    high = __reduce_max_sync(0xffffffffu, of->hi);
-  }
+  newest = __reduce_max_sync(0xffffffffu, peer(other)->newest);
+  low = __reduce_min_sync(0xffffffffu, peer(other)->lo);
+  high = __reduce_max_sync(0xffffffffu, peer(other)->hi);
 
   // Protected keys rank above every weight; the first histogram comes with the same pass.
   const long long recent_above = (long long)newest - a.recent;
   int shift = max(0, 32 - __clz(high - low) - 10);
   int mine = 0;
+#pragma unroll 4
   for (int t = tid; t < len; t += NT) {
-    const int32_t p = s_pos[t];
+    const int32_t p = pos[t];
     if (p < a.sink || (long long)p > recent_above) {
       s_rank[t] = kProtected;
       ++mine;
@@ -184,12 +197,12 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
   int left = 0, equal_before = 0, need = m;
   for (int turn = 0;; ++turn) {
     sync_all();
-    int* hist = sm.hist[turn & 1];
     if (turn == 0) {
-      const int p = __reduce_add_sync(0xffffffffu, lane < cluster ? peer(lane < cluster ? lane : 0)->n_protected : 0);
-      const int b = __reduce_add_sync(0xffffffffu, lane < part ? peer(lane < cluster ? lane : 0)->n_protected : 0);
+      const int x = peer(other)->n_protected;
+      const int p = __reduce_add_sync(0xffffffffu, lane < cluster ? x : 0);
+      const int b = __reduce_add_sync(0xffffffffu, lane < part ? x : 0);
       if (m <= p) {
-        left = m;
+        left = m < p ? m : -1;
         equal_before = b;
         break;
       }
@@ -202,10 +215,14 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
     constexpr int kPer = kBins / NT;
     int count[kPer], before[kPer], sum = 0;
 #pragma unroll
+    for (int i = 0; i < kPer; ++i) count[i] = 0;
+    for (int p = 0; p < cluster; ++p) {
+      const int* from = peer(p)->hist[turn & 1];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) count[i] += from[kBins - 1 - (tid * kPer + i)];
+    }
+#pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int bin = kBins - 1 - (tid * kPer + i);
-      count[i] = 0;
-      for (int p = 0; p < cluster; ++p) count[i] += peer(p)->hist[turn & 1][bin];
       before[i] = sum;
       sum += count[i];
     }
@@ -221,10 +238,10 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
       }
     }
     __syncthreads();
-    const int bin = sm.pick[0];
+    const int bin = sm.pick[0], inside = sm.pick[2];
     need = sm.pick[1];
     low += (uint32_t)bin << shift;
-    if (need == sm.pick[2]) {  // the whole interval stays
+    if (need == inside) {  // the whole interval stays
       top = low;
       left = -1;
       break;
@@ -232,141 +249,197 @@ __global__ void __launch_bounds__(NT) evict_kernel(Args a, int cluster, int keys
     if (shift == 0) {
       top = low;
       left = need;
-      equal_before = __reduce_add_sync(0xffffffffu, lane < part ? peer(lane < cluster ? lane : 0)->hist[turn & 1][bin] : 0);
+      equal_before = __reduce_add_sync(0xffffffffu, lane < part ? peer(other)->hist[turn & 1][bin] : 0);
       break;
     }
     const uint32_t width = 1u << shift;
+    if (inside <= kGather) {
+      for (int t = tid; t < len; t += NT) {
+        const uint32_t x = s_rank[t];
+        if (x != kProtected && x >= low && x - low < width) sm.cand[atomicAdd(&sm.n_cand, 1)] = x - low;
+      }
+      sync_all();
+      if (warp == 0) {
+        int at = 0, at_mine = 0;
+        for (int p = 0; p < cluster; ++p) {
+          const Shared* of = peer(p);
+          const int k = of->n_cand;
+          if (p == part) at_mine = at;
+          for (int i = lane; i < k; i += 32) sm.found[at + i] = of->cand[i];
+          at += k;
+        }
+        __syncwarp();
+        uint32_t v[kGather / 32];
+#pragma unroll
+        for (int i = 0; i < kGather / 32; ++i) v[i] = i * 32 + lane < at ? sm.found[i * 32 + lane] : 0;
+        auto at_least = [&](uint32_t x) {
+          int c = 0;
+#pragma unroll
+          for (int i = 0; i < kGather / 32; ++i) c += i * 32 + lane < at && v[i] >= x;
+          return (int)__reduce_add_sync(0xffffffffu, c);
+        };
+        uint32_t x = 0;  // the need-th largest, relative to the interval
+        for (int bit = shift - 1; bit >= 0; --bit)
+          if (at_least(x | 1u << bit) >= need) x |= 1u << bit;
+        int over = 0, equal = 0, ahead = 0;
+#pragma unroll
+        for (int i = 0; i < kGather / 32; ++i) {
+          if (i * 32 + lane >= at) continue;
+          over += v[i] > x;
+          equal += v[i] == x;
+          ahead += v[i] == x && i * 32 + lane < at_mine;
+        }
+        over = __reduce_add_sync(0xffffffffu, over);
+        equal = __reduce_add_sync(0xffffffffu, equal);
+        ahead = __reduce_add_sync(0xffffffffu, ahead);
+        if (lane == 0) {
+          sm.pick[0] = (int)(low + x);
+          sm.pick[1] = equal == need - over ? -1 : need - over;
+          sm.pick[2] = ahead;
+        }
+      }
+      __syncthreads();
+      top = (uint32_t)sm.pick[0];
+      left = sm.pick[1];
+      equal_before = sm.pick[2];
+      break;
+    }
     shift = max(0, shift - 10);
     int* next = sm.hist[(turn + 1) & 1];
     for (int t = tid; t < len; t += NT) {
-      const uint32_t x = s_rank[t] - low;
-      if (s_rank[t] != kProtected && s_rank[t] >= low && x < width) atomicAdd(&next[x >> shift], 1);
+      const uint32_t x = s_rank[t];
+      if (x != kProtected && x >= low && x - low < width) atomicAdd(&next[(x - low) >> shift], 1);
     }
-    (void)hist;
   }
 
-  // 3. Each warp's neighbouring slots.
-  const int seg = ((len + kWarps - 1) / kWarps + 31) & ~31;
-  const int w0 = min(warp * seg, len), w1 = min(w0 + seg, len);
-  const uint32_t lower = (1u << lane) - 1u;
+  // 3. What is kept, a bit per slot ...
+  const int words = (len + 31) / 32;
+#pragma unroll 4
+  for (int i = warp; i < words; i += kWarps) {
+    const int t = i * 32 + lane;
+    const uint32_t x = t < len ? s_rank[t] : 0;
+    const uint32_t k = __ballot_sync(0xffffffffu, t < len && m > 0 && (left < 0 ? x >= top : x > top));
+    const uint32_t q = __ballot_sync(0xffffffffu, t < len && x == top);
+    if (lane == 0) s_kept[i] = k, s_equal[i] = q;
+  }
+  __syncthreads();
+  const int each = (words + NT - 1) / NT;  // neighbouring words of a thread
+  const int i0 = min(tid * each, words), i1 = min(i0 + each, words);
   if (left >= 0) {
-    int eq = 0;
-    for (int t = w0 + lane; t < w1; t += 32) eq += s_rank[t] == top;
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) sm.warp_a[warp] = eq;
-    __syncthreads();
-    equal_before += __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_a[lane] : 0);
-  }
-  int holes = 0, moved = 0;
-  for (int t0 = w0; t0 < w1; t0 += 32) {
-    const int t = t0 + lane;
-    const uint32_t x = t < w1 ? s_rank[t] : 0;
-    bool kept;
-    if (left < 0) {
-      kept = t < w1 && x >= top;
-    } else {
-      const uint32_t eq = __ballot_sync(0xffffffffu, t < w1 && x == top);
-      kept = t < w1 && (x > top || (x == top && equal_before + __popc(eq & lower) < left));
-      equal_before += __popc(eq);
+    int eq = 0, total;
+    for (int i = i0; i < i1; ++i) eq += __popc(s_equal[i]);
+    int seen = equal_before + block_scan(eq, sm.warp_a, kWarps, &total);
+    for (int i = i0; i < i1; ++i) {
+      uint32_t q = s_equal[i], k = s_kept[i];
+      const int here = __popc(q);
+      if (seen + here <= left) {
+        k |= q;
+      } else {
+        for (int j = seen; j < left; ++j) {  // the lowest left - seen of them
+          k |= q & -q;
+          q &= q - 1;
+        }
+      }
+      seen += here;
+      s_kept[i] = k;
     }
-    if (t < w1) s_rank[t] = kept;
-    const bool under = lo + t < m;
-    holes += __popc(__ballot_sync(0xffffffffu, t < w1 && under && !kept));
-    moved += __popc(__ballot_sync(0xffffffffu, kept && !under));
   }
-  __syncthreads();
-  if (lane == 0) sm.warp_a[warp] = holes, sm.warp_b[warp] = moved;
-  __syncthreads();
-  int hole_at = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_a[lane] : 0);
-  int move_at = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_b[lane] : 0);
-  if (warp == kWarps - 1 && lane == 0) sm.counts[0] = hole_at + holes, sm.counts[1] = move_at + moved;
+  // ... and the row's lists.
+  int counts = 0;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t under = bits_below(lo + 32 * i, m), valid = bits_below(32 * i, len);
+    counts += __popc(~s_kept[i] & under & valid) + (__popc(s_kept[i] & ~under) << 16);
+  }
+  int block_counts;
+  const int before = block_scan(counts, sm.warp_a, kWarps, &block_counts);
+  if (tid == 0) sm.counts = block_counts;
   sync_all();
-  const Shared* of = peer(lane < cluster ? lane : 0);
-  const int c0 = lane < cluster ? of->counts[0] : 0, c1 = lane < cluster ? of->counts[1] : 0;
-  hole_at += __reduce_add_sync(0xffffffffu, lane < part ? c0 : 0);
-  move_at += __reduce_add_sync(0xffffffffu, lane < part ? c1 : 0);
-  const int moves = __reduce_add_sync(0xffffffffu, c1);
+  const int theirs = peer(other)->counts;
+  int hole_at = (before & 0xFFFF) + (int)__reduce_add_sync(0xffffffffu, lane < part ? theirs & 0xFFFF : 0);
+  int move_at = (int)((uint32_t)before >> 16) +
+                (int)__reduce_add_sync(0xffffffffu, lane < part ? (int)((uint32_t)theirs >> 16) : 0);
+  const int moves = (int)__reduce_add_sync(0xffffffffu, lane < cluster ? (int)((uint32_t)theirs >> 16) : 0);
   int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld;
   int32_t* movers = empties + a.list_ld;
-  for (int t0 = w0; t0 < w1; t0 += 32) {
-    const int t = t0 + lane;
-    const bool kept = t < w1 && s_rank[t];
-    const bool under = lo + t < m;
-    const uint32_t h = __ballot_sync(0xffffffffu, t < w1 && under && !kept);
-    const uint32_t v = __ballot_sync(0xffffffffu, kept && !under);
-    if (t < w1 && under && !kept) empties[hole_at + __popc(h & lower)] = lo + t;
-    if (kept && !under) movers[move_at + __popc(v & lower)] = lo + t;
-    hole_at += __popc(h);
-    move_at += __popc(v);
-    if (t < w1) {
-      if (under && kept) {
-        if (w_out != w) w_out[t] = w[t];
-        if (pos_out != pos) pos_out[t] = s_pos[t];
-      } else if (!under && !kept) {
-        w_out[t] = 0.f;
-        pos_out[t] = -1;
-      }
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t under = bits_below(lo + 32 * i, m), valid = bits_below(32 * i, len);
+    for (uint32_t x = ~s_kept[i] & under & valid; x; x &= x - 1) empties[hole_at++] = lo + 32 * i + __ffs(x) - 1;
+    for (uint32_t x = s_kept[i] & ~under; x; x &= x - 1) movers[move_at++] = lo + 32 * i + __ffs(x) - 1;
+  }
+  // What stays in place, and the slots beyond m that nothing moves from (the others are
+  // read once more by their move, which empties them).
+#pragma unroll 4
+  for (int t = tid; t < len; t += NT) {
+    const bool kept = s_kept[t >> 5] >> (t & 31) & 1;
+    if (lo + t < m) {
+      if (kept && w_out != w) w_out[t] = w[t];
+      if (kept && pos_out != pos) pos_out[t] = pos[t];
+    } else if (!kept) {
+      w_out[t] = 0.f;
+      pos_out[t] = -1;
     }
   }
-  __threadfence();
-  sync_all();  // the row's lists; after it no block reads another's shared memory or context length
-  if (part == 0 && tid == 0) a.ctx_out[r] = m;
+  if (part == 0 && tid == 0) {
+    a.ctx_out[r] = m;  // every block has read its length
+    a.counts[r] = moves;
+  }
+  if (cluster > 1) all.sync();  // no block leaves while another may read its counts
+}
 
-  // 4. The moves [first, last) of this block.
-  const int first = (int)((long long)moves * part / cluster), last = (int)((long long)moves * (part + 1) / cluster);
-  const int W = a.row_words, G = 2 * W, sub = tid % G, group = tid / G, groups = NT / G;
-  const float* w_row = a.w_in + r * a.ld;
-  const int32_t* pos_row = a.pos_in + r * a.ld;
-  float* w_to = a.w_out + r * a.ld;
-  int32_t* pos_to = a.pos_out + r * a.ld;
-  for (int i0 = first + group; i0 < last; i0 += groups * kMovesInFlight) {
-    int src[kMovesInFlight], dst[kMovesInFlight];
-    long long from[kMovesInFlight], to[kMovesInFlight];
+// Moves [128 i, 128 (i + 1)) of one row.  A thread each looks the pages up and moves weight
+// and position; then D / 16 lanes a key copy the codes, 16 bytes a lane, 4 keys at once.
+constexpr int kMoveThreads = 256;
+constexpr int kMoves = 128;
+
+template <int W>
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(Args a, int blocks_per_row) {
+  constexpr int G = 2 * W;
+  constexpr int kGroups = kMoveThreads / G;
+  constexpr int kFlight = 4;
+  __shared__ uint32_t s_from[kMoves], s_to[kMoves];
+  const int tid = threadIdx.x;
+  const int r = blockIdx.x / blocks_per_row;
+  const int first = (blockIdx.x - r * blocks_per_row) * kMoves;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int count = min(__ldcg(a.counts + r) - first, kMoves);
+  if (count <= 0) return;
+  if (tid < count) {
+    const int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld + first;
+    const int dst = __ldcg(empties + tid), src = __ldcg(empties + a.list_ld + tid);
+    const long long from = a.pages.slot(r, src), to = a.pages.slot(r, dst);
+    const bool ok = from >= 0 && to >= 0;
+    if (!ok) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+    s_from[tid] = ok ? (uint32_t)from : 0xffffffffu;
+    s_to[tid] = (uint32_t)to;
+    const long long row = r * a.ld;
+    const float w = a.w_in[row + src];
+    const int32_t p = a.pos_in[row + src];
+    a.w_out[row + dst] = w;
+    a.pos_out[row + dst] = p;
+    a.w_out[row + src] = 0.f;
+    a.pos_out[row + src] = -1;
+    if (ok && a.v_scale) a.v_scale[to] = a.v_scale[from];
+  }
+  __syncthreads();
+  const int sub = tid % G, group = tid / G;
+  const bool words = sub < W / 4;
+  for (int i0 = group; i0 < count; i0 += kGroups * kFlight) {
+    uint4 v[kFlight], k[kFlight];
+    uint32_t from[kFlight];
 #pragma unroll
-    for (int u = 0; u < kMovesInFlight; ++u) {
-      const int i = min(i0 + u * groups, last - 1);
-      src[u] = __ldcg(movers + i);
-      dst[u] = __ldcg(empties + i);
+    for (int u = 0; u < kFlight; ++u) {
+      const int i = i0 + u * kGroups;
+      from[u] = i < count ? s_from[i] : 0xffffffffu;
+      if (from[u] == 0xffffffffu) continue;
+      v[u] = *(reinterpret_cast<const uint4*>(a.v) + (size_t)from[u] * G + sub);
+      if (words) k[u] = *(reinterpret_cast<const uint4*>(a.k) + (size_t)from[u] * (W / 4) + sub);
     }
 #pragma unroll
-    for (int u = 0; u < kMovesInFlight; ++u) {
-      from[u] = a.pages.slot(r, src[u]);
-      to[u] = a.pages.slot(r, dst[u]);
-      if (from[u] < 0 || to[u] < 0) {
-        if (sub == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
-        from[u] = -1;
-      }
-    }
-    uint4 v[kMovesInFlight], k[kMovesInFlight];
-    float wv[kMovesInFlight], sv[kMovesInFlight];
-    int32_t pv[kMovesInFlight];
-    const bool words = sub < W / 4;
-#pragma unroll
-    for (int u = 0; u < kMovesInFlight; ++u) {
-      const long long at = max(from[u], 0LL);
-      v[u] = *(reinterpret_cast<const uint4*>(a.v + at * 32 * W) + sub);
-      if (words) k[u] = *(reinterpret_cast<const uint4*>(a.k + at * W) + sub);
-      if (sub == 0) {
-        wv[u] = w_row[src[u]];
-        pv[u] = pos_row[src[u]];
-        if (a.v_scale) sv[u] = a.v_scale[at];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kMovesInFlight; ++u) {
-      if (i0 + u * groups >= last) break;
-      if (from[u] >= 0) {
-        *(reinterpret_cast<uint4*>(a.v + to[u] * 32 * W) + sub) = v[u];
-        if (words) *(reinterpret_cast<uint4*>(a.k + to[u] * W) + sub) = k[u];
-        if (sub == 0 && a.v_scale) a.v_scale[to[u]] = sv[u];
-      }
-      if (sub == 0) {
-        w_to[dst[u]] = wv[u];
-        pos_to[dst[u]] = pv[u];
-        w_to[src[u]] = 0.f;
-        pos_to[src[u]] = -1;
-      }
+    for (int u = 0; u < kFlight; ++u) {
+      if (from[u] == 0xffffffffu) continue;
+      const size_t to = s_to[i0 + u * kGroups];
+      *(reinterpret_cast<uint4*>(a.v) + to * G + sub) = v[u];
+      if (words) *(reinterpret_cast<uint4*>(a.k) + to * (W / 4) + sub) = k[u];
     }
   }
 }
@@ -501,10 +574,12 @@ __global__ void __launch_bounds__(kLongThreads) evict_long_kernel(Args a) {
 
 inline long long list_ld(long long cap) { return cap / 2 + 1; }
 
-inline size_t scratch_bytes(long long n_kv, long long cap) { return (size_t)n_kv * 2 * list_ld(cap) * sizeof(int32_t); }
+// Lists first, then the counts.
+inline size_t lists_bytes(long long n_kv, long long cap) { return (size_t)n_kv * 2 * list_ld(cap) * sizeof(int32_t); }
+inline size_t scratch_bytes(long long n_kv, long long cap) { return lists_bytes(n_kv, cap) + (size_t)n_kv * sizeof(int32_t); }
 
 constexpr size_t kMaxSmem = 227 * 1024;
-constexpr int kBlockKeys = 8192;  // of a row per block, while 16 blocks do
+constexpr int kBlockKeys = 16384;  // of a row per block, while 16 blocks do
 
 inline cudaError_t setup() {
   cudaError_t e = cudaSuccess;
@@ -512,22 +587,25 @@ inline cudaError_t setup() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   };
-  set(reinterpret_cast<const void*>(evict_kernel<512>));
-  set(reinterpret_cast<const void*>(evict_kernel<1024>));
+  set(reinterpret_cast<const void*>(select_kernel<512, 4>));
+  set(reinterpret_cast<const void*>(select_kernel<1024, 2>));
   return e;
 }
 
-inline cudaError_t launch(const Args& a, cudaStream_t st) {
+inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
   const long long cap = (long long)a.pages.num_blocks * a.pages.block_size;
   int cluster = 1;
-  while (cluster < kMaxCluster && (cap + cluster - 1) / cluster > kBlockKeys) cluster *= 2;
-  const long long keys = ((cap + cluster - 1) / cluster + 31) / 32 * 32;
-  const size_t smem = sizeof(Shared) + (size_t)keys * 8;
+  auto part = [&](int c) { return ((cap + c - 1) / c + 31) / 32 * 32; };
+  while (cluster < kMaxCluster && part(cluster) > kBlockKeys) cluster *= 2;
+  // Few rows: more blocks a row while the device has room and a block keeps 4096 keys.
+  while (cluster < 8 && (long long)a.n_kv * cluster * 2 <= n_sm && part(cluster) >= 8192) cluster *= 2;
+  const long long keys = part(cluster);
+  const size_t smem = sizeof(Shared) + (size_t)keys * 4 + (size_t)keys / 32 * 8;
   if (smem > kMaxSmem) {
     evict_long_kernel<<<(unsigned)a.n_kv, kLongThreads, 0, st>>>(a);
     return cudaGetLastError();
   }
-  const int threads = keys > 4096 ? 1024 : 512;
+  const int threads = keys > 8192 ? 1024 : 512;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)a.n_kv * cluster));
   cfg.blockDim = dim3((unsigned)threads);
@@ -539,8 +617,25 @@ inline cudaError_t launch(const Args& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = threads == 1024 ? cudaLaunchKernelEx(&cfg, evict_kernel<1024>, a, cluster, (int)keys)
-                                        : cudaLaunchKernelEx(&cfg, evict_kernel<512>, a, cluster, (int)keys);
+  cudaError_t e = threads == 1024 ? cudaLaunchKernelEx(&cfg, select_kernel<1024, 2>, a, cluster, (int)keys)
+                                  : cudaLaunchKernelEx(&cfg, select_kernel<512, 4>, a, cluster, (int)keys);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // The most moves a row can have: its budget, or what lies beyond it.
+  const long long most = a.keep_rows ? cap / 2 : std::min<long long>(a.keep, cap - a.keep);
+  if (most <= 0) return cudaSuccess;
+  const int per_row = (int)((most + kMoves - 1) / kMoves);
+  cudaLaunchConfig_t move = {};
+  move.gridDim = dim3((unsigned)((long long)a.n_kv * per_row));
+  move.blockDim = dim3(kMoveThreads);
+  move.stream = st;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  move.attrs = pdl;
+  move.numAttrs = 1;
+  e = a.row_words == 8 ? cudaLaunchKernelEx(&move, move_kernel<8>, a, per_row)
+                       : cudaLaunchKernelEx(&move, move_kernel<4>, a, per_row);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 

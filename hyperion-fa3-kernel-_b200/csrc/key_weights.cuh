@@ -333,7 +333,11 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(Args a, ChunkArgs c, int 
   const int r = blockIdx.x / blocks_per_row;
   const int base = (blockIdx.x - r * blocks_per_row) * kThreads * 4 * kGroups;
   const int n = a.pages.context(__ldg(a.ctx_lens + r), a.err, false);
-  if (base >= n) return;
+  if (base >= n) {
+    // Even so: this grid ends after the one it depends on.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const float* in = a.in + r * a.ld;
   float x[kGroups][4];
 #pragma unroll

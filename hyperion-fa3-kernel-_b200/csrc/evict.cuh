@@ -46,9 +46,9 @@ struct Args {
 
 // Order-preserving image of a weight sum: -0 as +0, NaN below everything.
 __device__ __forceinline__ uint32_t rank_of(float w) {
-  if (w != w) return 0;
   const uint32_t b = __float_as_uint(w + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const uint32_t x = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return w != w ? 0 : x;
 }
 
 // ---------------------------------------------------------------------------
@@ -58,20 +58,23 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 //   1. Read weights and positions once; the row's newest position and the range of its
 //      ranks by way of distributed shared memory.
 //   2. The m-th largest rank, by histograms of kBins equal intervals of the range that is
-//      left (10 bits a turn), until an interval is kept whole or holds at most kGather
-//      ranks: those are gathered and one warp finds the rank among them bit by bit.  Sums
-//      of attention weights take one or two turns.
-//   3. A bit per slot says what is kept.  A thread turns a word of 32 slots into its part
-//      of the row's two lists (slots that empty below m, keys that move), in slot order.
+//      left (12 bits a turn), until an interval is kept whole or holds at most kGather
+//      ranks: those are gathered and each is counted against the others.  Sums of attention
+//      weights take one turn, now and then two.  So many intervals also keep the lanes of a
+//      warp from adding to the same one: with 1024, 4 to 5 of 32 met.
+//   3. A bit per slot says what is kept.  The counts of 32 slots are added up per word, and
+//      each warp writes its slots' places into the row's two lists (slots that empty below
+//      m, keys that move), in slot order.
 //
 // move_kernel: the moves of all rows, 128 a block, whichever row they belong to.
 // ---------------------------------------------------------------------------
-constexpr int kBins = 1024;
+constexpr int kBins = 4096;  // two 16-bit counts a word: a block has at most 52k keys
+constexpr int kBinBits = 12;
 constexpr int kGather = 256;
 constexpr int kMaxCluster = 16;
 
-struct Shared {
-  int hist[2][kBins];
+struct __align__(16) Shared {
+  uint32_t hist[2][kBins / 2];
   uint32_t cand[kGather];   // this block's ranks of the gathered interval, relative to it
   uint32_t found[kGather];  // the row's
   int n_cand;
@@ -102,14 +105,42 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int warps, int* to
   return before + inc - x;
 }
 
+// One more in interval `bin`.
+__device__ __forceinline__ void count_one(uint32_t* hist, uint32_t bin) { atomicAdd(hist + (bin >> 1), 1u << (16 * (bin & 1))); }
+
 // Bits of word `at` (slots at .. at + 31) that lie below `end`.
 __device__ __forceinline__ uint32_t bits_below(int at, int end) {
   const int k = end - at;
   return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
 }
 
+// Four neighbouring values, `n` of them real; one read or write where `vec`.
+template <typename V, typename T>
+__device__ __forceinline__ void load4(T (&x)[4], const T* p, int n, bool vec) {
+  if (vec && n >= 4) {
+    const V v = *reinterpret_cast<const V*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = j < n ? p[j] : T(0);
+  }
+}
+template <typename V, typename T>
+__device__ __forceinline__ void store4(T* p, const T (&x)[4], int n, bool vec) {
+  if (vec && n >= 4) {
+    V v;
+    v.x = x[0], v.y = x[1], v.z = x[2], v.w = x[3];
+    *reinterpret_cast<V*>(p) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = x[j];
+  }
+}
+
+// Each thread works on 4 neighbouring slots at a time; `vec`: the rows lie on 16 bytes.
 template <int NT, int kBlocks>
-__global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster, int keys) {
+__global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster, int keys, bool vec) {
   namespace cg = cooperative_groups;
   constexpr int kWarps = NT / 32;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -150,19 +181,30 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
   // 1. Ranks, newest position, range of the ranks.
   int newest = INT_MIN;
   uint32_t low = 0xffffffffu, high = 0;
-#pragma unroll 4
-  for (int t = tid; t < len; t += NT) {
-    const uint32_t x = rank_of(w[t]);
-    s_rank[t] = x;
-    newest = max(newest, pos[t]);
-    low = min(low, x);
-    high = max(high, x);
+#pragma unroll 2
+  for (int t = 4 * tid; t < len; t += 4 * NT) {
+    const int real = len - t;
+    float wv[4];
+    int32_t pv[4];
+    uint32_t x[4];
+    load4<float4>(wv, w + t, real, vec);
+    load4<int4>(pv, pos + t, real, vec);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = rank_of(wv[j]);
+      if (j < real) {
+        newest = max(newest, pv[j]);
+        low = min(low, x[j]);
+        high = max(high, x[j]);
+      }
+    }
+    *reinterpret_cast<uint4*>(s_rank + t) = make_uint4(x[0], x[1], x[2], x[3]);
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
   low = __reduce_min_sync(0xffffffffu, low);
   high = __reduce_max_sync(0xffffffffu, high);
   if (lane == 0) sm.warp_a[warp] = newest, sm.warp_lo[warp] = low, sm.warp_hi[warp] = high;
-  for (int i = tid; i < 2 * kBins; i += NT) (&sm.hist[0][0])[i] = 0;
+  for (int i = tid; i < kBins / 8; i += NT) reinterpret_cast<uint4*>(sm.hist[0])[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (warp == 0) {
     newest = __reduce_max_sync(0xffffffffu, lane < kWarps ? sm.warp_a[lane] : INT_MIN);
@@ -176,17 +218,25 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
   high = __reduce_max_sync(0xffffffffu, peer(other)->hi);
 
   // Protected keys rank above every weight; the first histogram comes with the same pass.
-  const long long recent_above = (long long)newest - a.recent;
-  int shift = max(0, 32 - __clz(high - low) - 10);
+  int shift = max(0, 32 - __clz(high - low) - kBinBits);
   int mine = 0;
-#pragma unroll 4
-  for (int t = tid; t < len; t += NT) {
-    const int32_t p = pos[t];
-    if (p < a.sink || (long long)p > recent_above) {
-      s_rank[t] = kProtected;
-      ++mine;
-    } else {
-      atomicAdd(&sm.hist[0][(s_rank[t] - low) >> shift], 1);
+#pragma unroll 2
+  for (int t = 4 * tid; t < len; t += 4 * NT) {
+    const int real = len - t;
+    int32_t pv[4];
+    load4<int4>(pv, pos + t, real, vec);
+    const uint4 v = *reinterpret_cast<const uint4*>(s_rank + t);
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= real) continue;
+      // newest - p may pass 2^31, not 2^32
+      if (pv[j] < a.sink || (uint32_t)newest - (uint32_t)pv[j] < (uint32_t)a.recent) {
+        s_rank[t + j] = kProtected;
+        ++mine;
+      } else {
+        count_one(sm.hist[0], (x[j] - low) >> shift);
+      }
     }
   }
   mine = __reduce_add_sync(0xffffffffu, mine);
@@ -207,34 +257,34 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
         break;
       }
       need = m - p;
-    } else {
-      // Nobody reads the other buffer any more.
-      for (int i = tid; i < kBins; i += NT) sm.hist[(turn + 1) & 1][i] = 0;
     }
-    // This thread's intervals, from the highest down.
+    // This thread's intervals, kPer neighbours; thread 0 has the highest.
     constexpr int kPer = kBins / NT;
-    int count[kPer], before[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) count[i] = 0;
+    static_assert(kPer >= 4, "a thread reads its intervals 4 at a time");
+    const int bin0 = kBins - kPer * (tid + 1);
+    int count[kPer] = {}, sum = 0;
     for (int p = 0; p < cluster; ++p) {
-      const int* from = peer(p)->hist[turn & 1];
+      const uint32_t* from = peer(p)->hist[turn & 1] + bin0 / 2;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) count[i] += from[kBins - 1 - (tid * kPer + i)];
+      for (int i = 0; i < kPer; i += 4) {
+        const uint2 x = *reinterpret_cast<const uint2*>(from + i / 2);
+        count[i] += x.x & 0xFFFF, count[i + 1] += x.x >> 16;
+        count[i + 2] += x.y & 0xFFFF, count[i + 3] += x.y >> 16;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      before[i] = sum;
-      sum += count[i];
-    }
+    for (int i = 0; i < kPer; ++i) sum += count[i];
     int total;
-    const int above = block_scan(sum, sm.warp_a, kWarps, &total);
+    int above = block_scan(sum, sm.warp_a, kWarps, &total);
+    if (above < need && need <= above + sum) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c0 = above + before[i];
-      if (c0 < need && need <= c0 + count[i]) {
-        sm.pick[0] = kBins - 1 - (tid * kPer + i);
-        sm.pick[1] = need - c0;
-        sm.pick[2] = count[i];
+      for (int i = kPer - 1; i >= 0; --i) {
+        if (above < need && need <= above + count[i]) {
+          sm.pick[0] = bin0 + i;
+          sm.pick[1] = need - above;
+          sm.pick[2] = count[i];
+        }
+        above += count[i];
       }
     }
     __syncthreads();
@@ -249,78 +299,88 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
     if (shift == 0) {
       top = low;
       left = need;
-      equal_before = __reduce_add_sync(0xffffffffu, lane < part ? peer(other)->hist[turn & 1][bin] : 0);
+      equal_before = __reduce_add_sync(0xffffffffu, lane < part ? (int)(peer(other)->hist[turn & 1][bin >> 1] >> (16 * (bin & 1)) & 0xFFFF) : 0);
       break;
     }
     const uint32_t width = 1u << shift;
     if (inside <= kGather) {
-      for (int t = tid; t < len; t += NT) {
-        const uint32_t x = s_rank[t];
-        if (x != kProtected && x >= low && x - low < width) sm.cand[atomicAdd(&sm.n_cand, 1)] = x - low;
+      for (int t = 4 * tid; t < len; t += 4 * NT) {
+        const uint4 v = *reinterpret_cast<const uint4*>(s_rank + t);
+        const uint32_t x[4] = {v.x - low, v.y - low, v.z - low, v.w - low};
+        if (min(min(x[0], x[1]), min(x[2], x[3])) >= width) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t + j < len && x[j] < width && x[j] + low != kProtected) sm.cand[atomicAdd(&sm.n_cand, 1)] = x[j];
       }
       sync_all();
-      if (warp == 0) {
-        int at = 0, at_mine = 0;
-        for (int p = 0; p < cluster; ++p) {
-          const Shared* of = peer(p);
-          const int k = of->n_cand;
-          if (p == part) at_mine = at;
-          for (int i = lane; i < k; i += 32) sm.found[at + i] = of->cand[i];
-          at += k;
+      // All blocks' candidates, in the order of the blocks, padded with zeros; a thread
+      // counts one of them.
+      int at = 0, ahead_end = 0;
+      for (int p = 0; p < cluster; ++p) {
+        const Shared* of = peer(p);
+        const int k = of->n_cand;
+        if (p == part) ahead_end = at;
+        if (tid < k) sm.found[at + tid] = of->cand[tid];
+        at += k;
+      }
+      if (tid < 4 && at + tid < kGather) sm.found[at + tid] = 0;
+      __syncthreads();
+      const uint32_t x = tid < at ? sm.found[tid] : 0;
+      const uint32_t first = sm.found[0];
+      if (__syncthreads_and(tid >= at || x == first)) {  // keys that nothing has looked at share a sum
+        if (tid == 0) sm.pick[0] = (int)first, sm.pick[1] = need;
+      } else if (warp * 32 < at) {
+        int over = 0, not_under = 0;
+#pragma unroll 4
+        for (int i = 0; i < (at + 3) / 4; ++i) {
+          const uint4 y = reinterpret_cast<const uint4*>(sm.found)[i];
+          over += (y.x > x) + (y.y > x) + (y.z > x) + (y.w > x);
+          not_under += (y.x >= x) + (y.y >= x) + (y.z >= x) + (y.w >= x);
         }
-        __syncwarp();
-        uint32_t v[kGather / 32];
-#pragma unroll
-        for (int i = 0; i < kGather / 32; ++i) v[i] = i * 32 + lane < at ? sm.found[i * 32 + lane] : 0;
-        auto at_least = [&](uint32_t x) {
-          int c = 0;
-#pragma unroll
-          for (int i = 0; i < kGather / 32; ++i) c += i * 32 + lane < at && v[i] >= x;
-          return (int)__reduce_add_sync(0xffffffffu, c);
-        };
-        uint32_t x = 0;  // the need-th largest, relative to the interval
-        for (int bit = shift - 1; bit >= 0; --bit)
-          if (at_least(x | 1u << bit) >= need) x |= 1u << bit;
-        int over = 0, equal = 0, ahead = 0;
-#pragma unroll
-        for (int i = 0; i < kGather / 32; ++i) {
-          if (i * 32 + lane >= at) continue;
-          over += v[i] > x;
-          equal += v[i] == x;
-          ahead += v[i] == x && i * 32 + lane < at_mine;
-        }
-        over = __reduce_add_sync(0xffffffffu, over);
-        equal = __reduce_add_sync(0xffffffffu, equal);
-        ahead = __reduce_add_sync(0xffffffffu, ahead);
-        if (lane == 0) {
-          sm.pick[0] = (int)(low + x);
-          sm.pick[1] = equal == need - over ? -1 : need - over;
-          sm.pick[2] = ahead;
+        if (x == 0) not_under = at;
+        if (tid < at && over < need && need <= not_under) {  // all such threads hold the same rank
+          sm.pick[0] = (int)x;
+          sm.pick[1] = need == not_under ? -1 : need - over;
         }
       }
       __syncthreads();
-      top = (uint32_t)sm.pick[0];
+      const uint32_t found = (uint32_t)sm.pick[0];
       left = sm.pick[1];
-      equal_before = sm.pick[2];
+      equal_before = __syncthreads_count(tid < ahead_end && x == found);
+      top = low + found;
       break;
     }
-    shift = max(0, shift - 10);
-    int* next = sm.hist[(turn + 1) & 1];
+    shift = max(0, shift - kBinBits);
+    // The other buffer's readers, in the turn before, are past this turn's sync.
+    uint32_t* next = sm.hist[(turn + 1) & 1];
+    for (int i = tid; i < kBins / 8; i += NT) reinterpret_cast<uint4*>(next)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
     for (int t = tid; t < len; t += NT) {
       const uint32_t x = s_rank[t];
-      if (x != kProtected && x >= low && x - low < width) atomicAdd(&next[(x - low) >> shift], 1);
+      if (x != kProtected && x >= low && x - low < width) count_one(next, (x - low) >> shift);
     }
   }
 
   // 3. What is kept, a bit per slot ...
   const int words = (len + 31) / 32;
-#pragma unroll 4
-  for (int i = warp; i < words; i += kWarps) {
-    const int t = i * 32 + lane;
-    const uint32_t x = t < len ? s_rank[t] : 0;
-    const uint32_t k = __ballot_sync(0xffffffffu, t < len && m > 0 && (left < 0 ? x >= top : x > top));
-    const uint32_t q = __ballot_sync(0xffffffffu, t < len && x == top);
-    if (lane == 0) s_kept[i] = k, s_equal[i] = q;
+  for (int t0 = 128 * warp; t0 < len; t0 += 4 * NT) {  // a warp: 4 words
+    const int t = t0 + 4 * lane, real = len - t;
+    const uint4 v = *reinterpret_cast<const uint4*>(s_rank + min(t, keys - 4));
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t k = 0, q = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      k |= (j < real && (left < 0 ? x[j] >= top : x[j] > top)) << j;
+      q |= (j < real && x[j] == top) << j;
+    }
+    k <<= 4 * (lane & 7), q <<= 4 * (lane & 7);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) k |= __shfl_xor_sync(0xffffffffu, k, o);
+    if (left >= 0) {
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) q |= __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if ((lane & 7) == 0 && real > 0) s_kept[t >> 5] = m > 0 ? k : 0, s_equal[t >> 5] = q;
   }
   __syncthreads();
   const int each = (words + NT - 1) / NT;  // neighbouring words of a thread
@@ -344,39 +404,71 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
       s_kept[i] = k;
     }
   }
-  // ... and the row's lists.
+  // ... and the row's lists: slots that empty | keys that move << 16, before each word.
   int counts = 0;
   for (int i = i0; i < i1; ++i) {
     const uint32_t under = bits_below(lo + 32 * i, m), valid = bits_below(32 * i, len);
     counts += __popc(~s_kept[i] & under & valid) + (__popc(s_kept[i] & ~under) << 16);
   }
   int block_counts;
-  const int before = block_scan(counts, sm.warp_a, kWarps, &block_counts);
-  if (tid == 0) sm.counts = block_counts;
-  sync_all();
-  const int theirs = peer(other)->counts;
-  int hole_at = (before & 0xFFFF) + (int)__reduce_add_sync(0xffffffffu, lane < part ? theirs & 0xFFFF : 0);
-  int move_at = (int)((uint32_t)before >> 16) +
-                (int)__reduce_add_sync(0xffffffffu, lane < part ? (int)((uint32_t)theirs >> 16) : 0);
-  const int moves = (int)__reduce_add_sync(0xffffffffu, lane < cluster ? (int)((uint32_t)theirs >> 16) : 0);
-  int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld;
-  int32_t* movers = empties + a.list_ld;
+  int before = block_scan(counts, sm.warp_a, kWarps, &block_counts);
   for (int i = i0; i < i1; ++i) {
     const uint32_t under = bits_below(lo + 32 * i, m), valid = bits_below(32 * i, len);
-    for (uint32_t x = ~s_kept[i] & under & valid; x; x &= x - 1) empties[hole_at++] = lo + 32 * i + __ffs(x) - 1;
-    for (uint32_t x = s_kept[i] & ~under; x; x &= x - 1) movers[move_at++] = lo + 32 * i + __ffs(x) - 1;
+    s_equal[i] = (uint32_t)before;  // the ties are settled
+    before += __popc(~s_kept[i] & under & valid) + (__popc(s_kept[i] & ~under) << 16);
   }
-  // What stays in place, and the slots beyond m that nothing moves from (the others are
-  // read once more by their move, which empties them).
-#pragma unroll 4
-  for (int t = tid; t < len; t += NT) {
-    const bool kept = s_kept[t >> 5] >> (t & 31) & 1;
-    if (lo + t < m) {
-      if (kept && w_out != w) w_out[t] = w[t];
-      if (kept && pos_out != pos) pos_out[t] = pos[t];
-    } else if (!kept) {
-      w_out[t] = 0.f;
-      pos_out[t] = -1;
+  if (tid == 0) sm.counts = block_counts;
+  sync_all();
+  const uint32_t theirs = (uint32_t)peer(other)->counts;
+  const int hole_at = (int)__reduce_add_sync(0xffffffffu, lane < part ? theirs & 0xFFFF : 0);
+  const int move_at = (int)__reduce_add_sync(0xffffffffu, lane < part ? theirs >> 16 : 0);
+  const int moves = (int)__reduce_add_sync(0xffffffffu, lane < cluster ? theirs >> 16 : 0);
+  int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld + hole_at;
+  int32_t* movers = a.lists + ((size_t)r * 2 + 1) * a.list_ld + move_at;
+  // Into other tensors, what stays is copied and all beyond m emptied; in place, what
+  // moves is still to be read, so its move empties it.  A slot that empties gets its key's
+  // values from the move.
+  const bool w_else = w_out != w, pos_else = pos_out != pos;
+  const int split = min(max(m - lo, 0), len);  // this block's slots below m
+  for (int t = 4 * tid; t < split; t += 4 * NT) {
+    const int real = split - t, bit0 = t & 31;
+    if (w_else) {
+      float x[4];
+      load4<float4>(x, w + t, real, vec);
+      store4<float4>(w_out + t, x, real, vec);
+    }
+    if (pos_else) {
+      int32_t x[4];
+      load4<int4>(x, pos + t, real, vec);
+      store4<int4>(pos_out + t, x, real, vec);
+    }
+    const uint32_t gone = ~s_kept[t >> 5] & bits_below(t - bit0, split);
+    uint32_t here = gone >> bit0 & 0xF;
+    if (here) {
+      int32_t* to = empties + (s_equal[t >> 5] & 0xFFFF) + __popc(gone & ((1u << bit0) - 1u));
+      for (; here; here &= here - 1) *to++ = lo + t + __ffs(here) - 1;
+    }
+  }
+  for (int t = (split & ~3) + 4 * tid; t < len; t += 4 * NT) {
+    const int bit0 = t & 31;
+    const uint32_t stay = s_kept[t >> 5] & ~bits_below(t - bit0, split);
+    uint32_t here = stay >> bit0 & 0xF;
+    if (t >= split && (here == 0 || (w_else && pos_else))) {
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      const int32_t none[4] = {-1, -1, -1, -1};
+      store4<float4>(w_out + t, zero, len - t, vec);
+      store4<int4>(pos_out + t, none, len - t, vec);
+    } else {
+#pragma unroll 1
+      for (int j = max(split - t, 0); j < min(len - t, 4); ++j) {
+        const bool moves_on = here >> j & 1;
+        if (w_else || !moves_on) w_out[t + j] = 0.f;
+        if (pos_else || !moves_on) pos_out[t + j] = -1;
+      }
+    }
+    if (here) {
+      int32_t* to = movers + (s_equal[t >> 5] >> 16) + __popc(stay & ((1u << bit0) - 1u));
+      for (; here; here &= here - 1) *to++ = lo + t + __ffs(here) - 1;
     }
   }
   if (part == 0 && tid == 0) {
@@ -386,62 +478,69 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
   if (cluster > 1) all.sync();  // no block leaves while another may read its counts
 }
 
-// Moves [128 i, 128 (i + 1)) of one row.  A thread each looks the pages up and moves weight
-// and position; then D / 16 lanes a key copy the codes, 16 bytes a lane, 4 keys at once.
+// Moves [kMoves i, kMoves (i + 1)) of one row.  A thread looks a move's pages up; D / 16
+// lanes copy a key's codes, 16 bytes each and kFlight keys at once; and while those are
+// under way a thread each takes a move's words, weight, position and slot scale, whose
+// destinations lie side by side.
 constexpr int kMoveThreads = 256;
-constexpr int kMoves = 128;
+constexpr int kFlight = 4;
 
 template <int W>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(Args a, int blocks_per_row) {
   constexpr int G = 2 * W;
   constexpr int kGroups = kMoveThreads / G;
-  constexpr int kFlight = 4;
+  constexpr int kMoves = kGroups * kFlight;
+  constexpr uint32_t kNoRow = 0xffffffffu;
   __shared__ uint32_t s_from[kMoves], s_to[kMoves];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, sub = tid % G, group = tid / G;
   const int r = blockIdx.x / blocks_per_row;
   const int first = (blockIdx.x - r * blocks_per_row) * kMoves;
+  const int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int count = min(__ldcg(a.counts + r) - first, kMoves);
   if (count <= 0) return;
+  int src = 0, dst = 0;
+  uint32_t from = kNoRow, to = kNoRow;
   if (tid < count) {
-    const int32_t* empties = a.lists + (size_t)r * 2 * a.list_ld + first;
-    const int dst = __ldcg(empties + tid), src = __ldcg(empties + a.list_ld + tid);
-    const long long from = a.pages.slot(r, src), to = a.pages.slot(r, dst);
-    const bool ok = from >= 0 && to >= 0;
-    if (!ok) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
-    s_from[tid] = ok ? (uint32_t)from : 0xffffffffu;
-    s_to[tid] = (uint32_t)to;
+    dst = __ldcg(empties + first + tid);
+    src = __ldcg(empties + a.list_ld + first + tid);
+    from = (uint32_t)a.pages.slot(r, src);
+    to = (uint32_t)a.pages.slot(r, dst);
+    if (from == kNoRow || to == kNoRow) {
+      raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+      from = kNoRow;
+    }
+  }
+  if (tid < kMoves) s_from[tid] = from, s_to[tid] = to;
+  __syncthreads();
+  uint4 v[kFlight];
+  uint32_t at[kFlight];
+#pragma unroll
+  for (int u = 0; u < kFlight; ++u) {
+    at[u] = s_from[u * kGroups + group];
+    if (at[u] != kNoRow) v[u] = *(reinterpret_cast<const uint4*>(a.v) + (size_t)at[u] * G + sub);
+  }
+  if (tid < count) {
     const long long row = r * a.ld;
     const float w = a.w_in[row + src];
     const int32_t p = a.pos_in[row + src];
+    if (from != kNoRow) {
+      uint4 k[W / 4];
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) k[i] = *(reinterpret_cast<const uint4*>(a.k) + (size_t)from * (W / 4) + i);
+      const float scale = a.v_scale ? a.v_scale[from] : 0.f;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) *(reinterpret_cast<uint4*>(a.k) + (size_t)to * (W / 4) + i) = k[i];
+      if (a.v_scale) a.v_scale[to] = scale;
+    }
     a.w_out[row + dst] = w;
     a.pos_out[row + dst] = p;
-    a.w_out[row + src] = 0.f;
-    a.pos_out[row + src] = -1;
-    if (ok && a.v_scale) a.v_scale[to] = a.v_scale[from];
+    if (a.w_out == a.w_in) a.w_out[row + src] = 0.f;
+    if (a.pos_out == a.pos_in) a.pos_out[row + src] = -1;
   }
-  __syncthreads();
-  const int sub = tid % G, group = tid / G;
-  const bool words = sub < W / 4;
-  for (int i0 = group; i0 < count; i0 += kGroups * kFlight) {
-    uint4 v[kFlight], k[kFlight];
-    uint32_t from[kFlight];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      const int i = i0 + u * kGroups;
-      from[u] = i < count ? s_from[i] : 0xffffffffu;
-      if (from[u] == 0xffffffffu) continue;
-      v[u] = *(reinterpret_cast<const uint4*>(a.v) + (size_t)from[u] * G + sub);
-      if (words) k[u] = *(reinterpret_cast<const uint4*>(a.k) + (size_t)from[u] * (W / 4) + sub);
-    }
-#pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      if (from[u] == 0xffffffffu) continue;
-      const size_t to = s_to[i0 + u * kGroups];
-      *(reinterpret_cast<uint4*>(a.v) + to * G + sub) = v[u];
-      if (words) *(reinterpret_cast<uint4*>(a.k) + to * (W / 4) + sub) = k[u];
-    }
-  }
+  for (int u = 0; u < kFlight; ++u)
+    if (at[u] != kNoRow) *(reinterpret_cast<uint4*>(a.v) + (size_t)s_to[u * kGroups + group] * G + sub) = v[u];
 }
 
 // ---------------------------------------------------------------------------
@@ -587,6 +686,7 @@ inline cudaError_t setup() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   };
+  set(reinterpret_cast<const void*>(select_kernel<256, 4>));
   set(reinterpret_cast<const void*>(select_kernel<512, 4>));
   set(reinterpret_cast<const void*>(select_kernel<1024, 2>));
   return e;
@@ -605,7 +705,7 @@ inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
     evict_long_kernel<<<(unsigned)a.n_kv, kLongThreads, 0, st>>>(a);
     return cudaGetLastError();
   }
-  const int threads = keys > 8192 ? 1024 : 512;
+  const int threads = keys > 8192 ? 1024 : keys > 4608 ? 512 : 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)a.n_kv * cluster));
   cfg.blockDim = dim3((unsigned)threads);
@@ -617,14 +717,17 @@ inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = threads == 1024 ? cudaLaunchKernelEx(&cfg, select_kernel<1024, 2>, a, cluster, (int)keys)
-                                  : cudaLaunchKernelEx(&cfg, select_kernel<512, 4>, a, cluster, (int)keys);
+  auto on16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool vec = a.ld % 4 == 0 && on16(a.w_in) && on16(a.w_out) && on16(a.pos_in) && on16(a.pos_out);
+  auto kernel = threads == 1024 ? select_kernel<1024, 2> : threads == 512 ? select_kernel<512, 4> : select_kernel<256, 4>;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, cluster, (int)keys, vec);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // The most moves a row can have: its budget, or what lies beyond it.
   const long long most = a.keep_rows ? cap / 2 : std::min<long long>(a.keep, cap - a.keep);
   if (most <= 0) return cudaSuccess;
-  const int per_row = (int)((most + kMoves - 1) / kMoves);
+  const int moves = kMoveThreads / (2 * a.row_words) * kFlight;  // of a block
+  const int per_row = (int)((most + moves - 1) / moves);
   cudaLaunchConfig_t move = {};
   move.gridDim = dim3((unsigned)((long long)a.n_kv * per_row));
   move.blockDim = dim3(kMoveThreads);

@@ -22,7 +22,7 @@ INCLUDE = os.path.join(REPO, "include")
 
 SOURCES = ["capi.cu"]
 HEADERS = ["common.cuh", "row_kernel.cuh", "row_group_kernel.cuh", "row_mma_kernel.cuh", "tile_kernel.cuh", "tcgen05.cuh", "kv_write.cuh",
-           "cache_pages.cuh", "rope_write.cuh", "key_weights.cuh", "evict.cuh", "launch_table.h"]
+           "cache_pages.cuh", "rope_write.cuh", "key_weights.cuh", "key_weights_window.cuh", "evict.cuh", "launch_table.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

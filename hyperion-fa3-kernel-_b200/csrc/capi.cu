@@ -22,7 +22,7 @@
 #include "tile_kernel.cuh"
 #include "kv_write.cuh"
 #include "rope_write.cuh"
-#include "key_weights.cuh"
+#include "key_weights_window.cuh"
 #include "evict.cuh"
 #include "launch_table.h"
 
@@ -127,6 +127,8 @@ int get_dev(const DevInfo** out) {
       di.tile_why = why;
       cudaGetLastError();
     }
+    e = hyp::kweights::setup();
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(key weights)");
     e = hyp::evict::setup();
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(eviction)");
     di.mma_ok = hyp::rmma::setup(di.mma_ctas, di.mma_smem) == cudaSuccess && di.mma_ctas > 0;
@@ -728,9 +730,14 @@ extern "C" int hyperion_rope_cache_write(const hyperion_rope_write_args* x, void
 extern "C" size_t hyperion_key_weights_scratch_bytes(int32_t n_kv, int32_t kv_group, int32_t n_q, int32_t head_dim,
                                                      int32_t block_size, int32_t num_blocks) {
   if (n_kv < 1 || kv_group < 1 || n_q < 1 || block_size < 1 || num_blocks < 1) return 0;
-  const hyp::kweights::Plan p =
-      hyp::kweights::plan(n_kv, (long long)kv_group * n_q, head_dim, (long long)block_size * num_blocks);
-  return p.dist_bytes + p.part_bytes;
+  // Whatever inv_sqrt_d will be.
+  size_t most = 0;
+  for (const bool flat : {false, true}) {
+    const hyp::kweights::Plan p =
+        hyp::kweights::plan(n_kv, (long long)kv_group * n_q, head_dim, (long long)block_size * num_blocks, flat);
+    most = std::max(most, p.dist_bytes + p.part_bytes);
+  }
+  return most;
 }
 
 extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* x, void* workspace,
@@ -761,9 +768,13 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
   if (x->scratch == nullptr || !aligned(x->scratch, 16))
     return fail(HYPERION_ERR_WORKSPACE, "scratch missing or not 16-byte aligned");
   const hyp::kweights::Plan p = hyp::kweights::plan(x->n_kv, (long long)x->kv_group * x->n_q, x->head_dim,
-                                                    (long long)x->block_size * x->num_blocks);
+                                                    (long long)x->block_size * x->num_blocks,
+                                                    hyp::kweights::is_flat(x->inv_sqrt_d, x->head_dim));
   if (x->scratch_bytes < p.dist_bytes + p.part_bytes)
     return fail(HYPERION_ERR_WORKSPACE, "scratch smaller than hyperion_key_weights_scratch_bytes()");
+  const DevInfo* di = nullptr;  // sets the kernels up on their first use on a device
+  rc = get_dev(&di);
+  if (rc) return rc;
   hyp::kweights::Args a;
   a.q = x->q;
   a.k = x->k_cache;

@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(Args a, ChunkArgs c, int 
 }
 
 // ---------------------------------------------------------------------------
-// Any number of queries: two kernels, with each query's best and 1 / l between them.
+// Many queries at a scale beyond kFlat: two kernels on the CUDA cores, with each query's
+// best and 1 / l between them.  (At the usual scales: key_weights_window.cuh.)
 // ---------------------------------------------------------------------------
 // One block per query row: the least distance and the sum of E over its keys.
 template <int D>
@@ -519,89 +520,6 @@ __global__ void __launch_bounds__(kThreads) window_sum_kernel(Args a, int blocks
     }
   }
   a.out[r * a.ld + t] = fmaf(a.decay, a.in[r * a.ld + t], sum);
-}
-
-constexpr int kSms = 148;  // of a B200; the plan, and so the scratch, does not depend on the device
-
-// What a call launches and the scratch it needs.
-struct Plan {
-  bool few = false;  // the two streaming kernels; else the window kernels
-  int unroll = 1, groups = 1;
-  ChunkArgs c = {};
-  size_t dist_bytes = 0, part_bytes = 0;  // at the front of the scratch, distances first
-};
-
-inline Plan plan(long long n_kv, long long rows, int head_dim, long long cap) {
-  Plan p;
-  p.few = rows <= kMaxBatches * kBatch;
-  if (!p.few) {
-    p.part_bytes = (size_t)(n_kv * rows) * sizeof(int2);
-    return p;
-  }
-  const long long keys = n_kv * cap;
-  // 8 keys a thread where that still gives every SM its blocks, else one.
-  p.unroll = keys >= 2LL * kSms * kThreads * 8 ? 8 : 1;
-  p.groups = p.unroll == 8 ? 2 : 1;
-  p.c.batches = (int)((rows + kBatch - 1) / kBatch);
-  const long long chunk = (long long)kThreads * p.unroll;
-  p.c.chunks = (int)((cap + chunk - 1) / chunk);
-  const long long whole = (cap + 8 * kThreads - 1) / (8 * kThreads) * (8 * kThreads);
-  p.c.dist_ld = (int)whole;
-  p.dist_bytes = (size_t)n_kv * p.c.batches * whole * (head_dim == 256 ? 8 : 4);
-  p.part_bytes = (size_t)n_kv * p.c.chunks * p.c.batches * kBatch * sizeof(int2);
-  return p;
-}
-
-template <int D, bool kFlat>
-inline cudaError_t launch_few(const Args& a, Plan p, uint8_t* scratch, cudaStream_t st) {
-  const long long cap = (long long)a.pages.num_blocks * a.pages.block_size;
-  p.c.dist = scratch;
-  p.c.part = reinterpret_cast<int2*>(scratch + p.dist_bytes);
-  const unsigned grid = (unsigned)((long long)a.n_kv * p.c.chunks);
-  if (p.unroll == 8) {
-    score_kernel<D, kFlat, D == 128 ? 4 : 2, D == 128 ? 2 : 4><<<grid, kThreads, 0, st>>>(a, p.c);
-  } else {
-    score_kernel<D, kFlat, 1, 1><<<grid, kThreads, 0, st>>>(a, p.c);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const long long block = 4LL * kThreads * p.groups;
-  const int per_row = (int)((cap + block - 1) / block);
-  const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.in) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)a.n_kv * per_row));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  auto kernel = p.groups == 2 ? sum_kernel<D, kFlat, 2> : sum_kernel<D, kFlat, 1>;
-  e = cudaLaunchKernelEx(&cfg, kernel, a, p.c, kThreads * p.unroll, per_row, vec);
-  return e == cudaSuccess ? cudaGetLastError() : e;
-}
-
-template <int D>
-inline cudaError_t launch_d(Args a, uint8_t* scratch, cudaStream_t st) {
-  const long long rows = (long long)a.kv_group * a.n_q;
-  const long long cap = (long long)a.pages.num_blocks * a.pages.block_size;
-  const Plan p = plan(a.n_kv, rows, D, cap);
-  if (p.few)
-    return 2.f * std::fabs(a.inv_sqrt_d) * D <= -kExpClamp ? launch_few<D, true>(a, p, scratch, st)
-                                                           : launch_few<D, false>(a, p, scratch, st);
-  a.stats = reinterpret_cast<int2*>(scratch);
-  const int per_row = (int)((cap + kThreads - 1) / kThreads);
-  window_stats_kernel<D><<<(unsigned)(a.n_kv * rows), kThreads, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  window_sum_kernel<D><<<(unsigned)(a.n_kv * (long long)per_row), kThreads, 0, st>>>(a, per_row);
-  return cudaGetLastError();
-}
-
-inline cudaError_t launch(const Args& a, int head_dim, uint8_t* scratch, cudaStream_t st) {
-  return head_dim == 256 ? launch_d<256>(a, scratch, st) : launch_d<128>(a, scratch, st);
 }
 
 }  // namespace kweights

@@ -327,6 +327,16 @@ def test_weights_short_windows_partly_outside_the_rows(hyperion, group, n_q, cau
         _weights_check(hyperion, c, causal=causal, first=np.array(first, np.int32), n_q=n_q)
 
 
+@pytest.mark.parametrize("D, group, n_q, causal", [(128, 4, 70, True), (128, 2, 64, True), (128, 3, 43, False), (256, 5, 60, True)])
+def test_weights_windows_over_many_tiles_and_chunks(hyperion, D, group, n_q, causal):
+    lens = [5000, 2048, 2049, 300, 129, 4100]
+    c = _weights_case(lens, 1, group, D, block=16, seq_q=5000, seed=group)
+    first = (c["ctx"] - n_q + (0 if causal else 5000 - c["ctx"])).astype(np.int32)
+    _weights_check(hyperion, c, causal=causal, first=first, n_q=n_q, decay=0.5)
+    c["table"][0, 7], c["table"][1, 127], c["table"][5, 200] = -1, 1 << 30, -5
+    _weights_check(hyperion, c, causal=causal, first=first, n_q=n_q, err=hyperion.DEVERR_BAD_BLOCK)
+
+
 @pytest.mark.parametrize("D", [128, 256])
 def test_weights_many_rows_of_short_and_long_contexts(hyperion, D):
     """Enough keys for the blocks of many keys a thread, ends inside and between them."""

@@ -12,10 +12,14 @@
 //   kSum true    rows are keys, columns queries (the two operands change places): each
 //                thread sums E / l over the queries, for the key's weight.
 //
-// E comes from the table of key_weights.cuh by its bits: 2^23 + 4 p + the table's address is
-// exact in f32, so one FMA on the score leaves the address of E[p] in the low mantissa bits.
-// The exponential unit would take a warp instruction every 8 cycles of a sub-partition, the
-// table one every 4.
+// Here E = exp(inv_sqrt_d s), relative to a score of 0: within kFlat's bound it stays between
+// e^-40 and e^40, and typical exponents are small, so their rounding is too.  It is computed
+// in two ways side by side, because either alone would hold the kernel up.  Some columns
+// take 2^x on the exponential unit (a warp instruction every 2 cycles of an SM); the others
+// read a table in shared memory (one every cycle, beside the 1 / l of each column, which
+// costs as much again).  The table's address is one FMA away: in units of the smallest f32,
+// 2^-149, a subnormal number's bits are its value, so s times -2, plus 2 D and the table's
+// address, is the address of E[p] exactly.
 //
 // The two accumulators of a key tile (128 columns each, two blocks on an SM) are computed
 // and read in turn: while the threads read one, the tensor core fills the other, and the
@@ -47,7 +51,7 @@ struct WindowSmem {
   float e[D + 4];
   alignas(16) uint16_t mask[2][8];  // keys of each tile that exist
   int end[kWinQueries];             // keys each query sees, INT_MAX for a place without a query
-  float inv[kWinQueries];           // 1 / l, 0 for a place without a query
+  alignas(16) float inv[kWinQueries];  // 1 / l, 0 for a place without a query
   float half[2][128];               // sums of the upper 64 columns
   float out[kWinThreads * 8];       // the chunk's key sums (at most 16 tiles)
   int min_end;
@@ -91,8 +95,57 @@ __device__ __forceinline__ void expand_half(const HalfRow<D>& h, uint32_t tile, 
 
 __device__ __forceinline__ float shared_f32(uint32_t at) {
   float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
+}
+
+constexpr uint32_t kUnitSum = 0x6D, kUnitL = 0x49;
+
+// Sum over 64 accumulator columns of E (kSum: E / l of the column's query).  Masked: column i
+// counts where bit i of `on` is set.
+template <bool kSum, bool kMasked>
+__device__ __forceinline__ float sum_columns(uint32_t s_col, float e_bias, float x_mul, const float* inv, uint64_t on) {
+  // Of 8 column pairs, those that go to the exponential unit: 5 beside the reads of 1 / l, 3
+  // without.
+  constexpr uint32_t kUnit = kSum ? kUnitSum : kUnitL;
+  const float kMinusTwo = __uint_as_float(0x80000002u);  // -2 x 2^-149
+  float2 acc[2] = {};
+#pragma unroll
+  for (int cc = 0; cc < 64; cc += 32) {
+    uint32_t v[2][16];
+    tc::ld16(s_col + cc, v[0]);
+    tc::ld16(s_col + cc + 16, v[1]);
+    tc::ld_wait_regs(v[0]);
+    tc::ld_wait_regs(v[1]);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      float4 scale = make_float4(1.f, 1.f, 1.f, 1.f);
+      if (kSum) scale = *reinterpret_cast<const float4*>(inv + cc + i);
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float2 sc = make_float2(__uint_as_float(v[i / 16][i % 16 + j]), __uint_as_float(v[i / 16][i % 16 + j + 1]));
+        float2 w;
+        if (kUnit >> ((i + j) / 2 % 8) & 1) {
+          const float2 x = __fmul2_rn(sc, make_float2(x_mul, x_mul));
+          w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+        } else {
+          const float2 at = __ffma2_rn(sc, make_float2(kMinusTwo, kMinusTwo), make_float2(e_bias, e_bias));
+          w = make_float2(shared_f32(__float_as_uint(at.x)), shared_f32(__float_as_uint(at.y)));
+        }
+        if (kMasked) {
+          if (!(on >> (cc + i + j) & 1)) w.x = 0.f;
+          if (!(on >> (cc + i + j + 1) & 1)) w.y = 0.f;
+        }
+        if (kSum) {
+          acc[j / 2] = __ffma2_rn(w, j ? make_float2(scale.z, scale.w) : make_float2(scale.x, scale.y), acc[j / 2]);
+        } else {
+          acc[j / 2] = __fadd2_rn(acc[j / 2], w);
+        }
+      }
+    }
+  }
+  const float2 all = __fadd2_rn(acc[0], acc[1]);
+  return all.x + all.y;
 }
 
 template <int D, bool kSum>
@@ -128,10 +181,7 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
     tc::tmem_alloc(&sm.tmem_base, kWinTmemCols);
     tc::tmem_relinquish();
   }
-  {  // E, reversed where the best score has the greatest popcount
-    const float step = 2.f * fabsf(a.inv_sqrt_d);
-    for (int j = tid; j <= D; j += kWinThreads) sm.e[j] = expf(-step * (a.inv_sqrt_d < 0.f ? D - j : j));
-  }
+  for (int j = tid; j <= D; j += kWinThreads) sm.e[j] = expf(a.inv_sqrt_d * (float)(D - 2 * j));
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -154,7 +204,8 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   // This thread's accumulator row and 64 of its columns.
   const uint32_t s_col = tmem + ((uint32_t)(warp & 3) << 21) + 64u * (warp >> 2);
   const int lane_row = 32 * (warp & 3) + lane, col0 = 64 * (warp >> 2);
-  const float e_bias = 8388608.f + 2.f * D + (float)smem_u32(sm.e);
+  const float x_mul = a.inv_sqrt_d * kLog2e;
+  const float e_bias = __uint_as_float(2u * D + smem_u32(sm.e));  // x 2^-149
 
   auto key_slot = [&](int t) { return t < k1 ? a.pages.slot(r, t) : -1LL; };
   auto load_key = [&](long long slot) { return load_half<D>(a.k + max(slot, 0LL) * W, half); };
@@ -167,49 +218,55 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
     bits = (bits | (bits >> 8)) & 0xFFFFu;
     if (lane == 0) sm.mask[buf][warp] = (uint16_t)bits;
   };
+  auto flag_key = [&](long long slot, int t) {
+    if (slot < 0 && t < k1 && half == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+  };
 
   uint32_t turn0 = 0, turn1 = 0;  // uses of each accumulator so far
   const int group0 = kSum ? 0 : in_row - chunk * c.groups, group1 = kSum ? c.groups : group0 + 1;
   for (int group = group0; group < group1; ++group) {
     const int q0 = group * kWinQueries;
     const int two = rows - q0 > 128 ? 2 : 1;  // accumulators in use
-    // The group's queries: how far each sees, 1 / l, and their bytes.
+    // The first two key tiles on their way, then the group's queries: how far each sees,
+    // 1 / l, and their bytes.
+    long long slot = key_slot(k0 + row), next_slot = key_slot(k0 + kWinKeys + row);
+    flag_key(slot, k0 + row);
+    flag_key(next_slot, k0 + kWinKeys + row);
+    HalfRow<D> h = load_key(slot);
+    HalfRow<D> h2 = load_key(next_slot);
+    HalfRow<D> hq[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int i = q0 + s * 128 + row;
+      long long at = 0;
+      const bool real = i < rows && query_of(a, r, i, n, &at) > 0;
+      hq[s] = load_half<D>(a.q + (real ? at : 0) * W, half);
+    }
     long long q_row = 0;
     const int end = q0 + tid < rows ? query_of(a, r, q0 + tid, n, &q_row) : 0;
     sm.end[tid] = end > 0 ? end : INT_MAX;
     if (tid == 0) sm.min_end = INT_MAX;
+    put_key(h, slot, 0);
+    put_key(h2, next_slot, 1);
+    expand_half<D>(hq[0], q_tile, row, half);
+    if (two == 2) expand_half<D>(hq[1], q_tile + kTile, row, half);
+    next_slot = key_slot(k0 + 2 * kWinKeys + row);
+    tc::fence_proxy_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      issue(0, 0);
+      if (two == 2) issue(1, 0);
+    }
+    const int least = __reduce_min_sync(0xffffffffu, end > 0 ? end : INT_MAX);
+    if (lane == 0) atomicMin(&sm.min_end, least);
     if (kSum) {
       if (group == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
       float l = 0.f;
       const int used = (n + c.tiles * kWinKeys - 1) / (c.tiles * kWinKeys);
       const float* part = c.part + ((size_t)r * c.chunks * c.groups + group) * kWinQueries + tid;
+#pragma unroll 4
       for (int j = 0; j < used; ++j) l += __ldcg(part + (size_t)j * c.groups * kWinQueries);
       sm.inv[tid] = end > 0 && l > 0.f ? 1.f / l : 0.f;
-    }
-#pragma unroll 1
-    for (int s = 0; s < two; ++s) {
-      const int i = q0 + s * 128 + row;
-      long long at = 0;
-      const bool real = i < rows && query_of(a, r, i, n, &at) > 0;
-      const HalfRow<D> h = load_half<D>(a.q + (real ? at : 0) * W, half);
-      expand_half<D>(h, q_tile + s * kTile, row, half);
-    }
-    // The first two key tiles.
-    long long slot = key_slot(k0 + row), next_slot = key_slot(k0 + kWinKeys + row);
-    if (slot < 0 && k0 + row < k1 && half == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
-    if (next_slot < 0 && k0 + kWinKeys + row < k1 && half == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
-    HalfRow<D> h = load_key(slot);
-    HalfRow<D> h2 = load_key(next_slot);
-    put_key(h, slot, 0);
-    put_key(h2, next_slot, 1);
-    next_slot = key_slot(k0 + 2 * kWinKeys + row);
-    tc::fence_proxy_async_smem();
-    __syncthreads();
-    const int least = __reduce_min_sync(0xffffffffu, sm.end[tid]);
-    if (lane == 0) atomicMin(&sm.min_end, least);
-    if (tid == 0) {
-      issue(0, 0);
-      if (two == 2) issue(1, 0);
     }
     __syncthreads();
     const int min_end = sm.min_end;
@@ -222,7 +279,7 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
       slot = next_slot;
       const bool more = g + 2 < tiles;
       if (more) {
-        if (slot < 0 && kb + 2 * kWinKeys + row < k1 && half == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+        flag_key(slot, kb + 2 * kWinKeys + row);
         h = load_key(slot);
         next_slot = key_slot(kb + 3 * kWinKeys + row);
       }
@@ -238,55 +295,29 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
         mbar_wait(&sm.ready[s], (s ? turn1 : turn0) & 1, &sm.ctl, a.err);
         (s ? turn1 : turn0)++;
         tc::fence_after_sync();
-        const int my_end = kSum ? 0 : sm.end[s * 128 + lane_row];
-        const int t = kb + lane_row;  // kSum: this thread's key
-        float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 1
-        for (int cc = 0; cc < 64; cc += 32) {
-          uint32_t v[2][16];
-          tc::ld16(s_col + 128u * s + cc, v[0]);
-          tc::ld16(s_col + 128u * s + cc + 16, v[1]);
-          tc::ld_wait_regs(v[0]);
-          tc::ld_wait_regs(v[1]);
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int col = col0 + cc + 16 * b;
-            // Columns this row pairs with: all, or those that exist and are seen.
-            uint32_t on = 0xFFFFu;
-            if (!plain) {
-              if (kSum) {
-                on = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) on |= (t < sm.end[s * 128 + col + i] ? 1u : 0u) << i;
-              } else {
-                const int lim = my_end - (kb + col);
-                on = (mk[col >> 5] >> (col & 16)) & (lim >= 16 ? 0xFFFFu : lim <= 0 ? 0u : (1u << lim) - 1u);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float2 f = __ffma2_rn(make_float2(__uint_as_float(v[b][i]), __uint_as_float(v[b][i + 1])),
-                                          make_float2(-2.f, -2.f), make_float2(e_bias, e_bias));
-              float2 w = make_float2(shared_f32(__float_as_uint(f.x) & 0x7FFFFFu), shared_f32(__float_as_uint(f.y) & 0x7FFFFFu));
-              if (!plain) {
-                if (!(on >> i & 1)) w.x = 0.f;
-                if (!(on >> (i + 1) & 1)) w.y = 0.f;
-              }
-              if (kSum) {
-                const float2 inv = *reinterpret_cast<const float2*>(&sm.inv[s * 128 + col + i]);
-                acc = __ffma2_rn(w, inv, acc);
-              } else {
-                acc = __fadd2_rn(acc, w);
-              }
-            }
+        const uint32_t col = s_col + 128u * s;
+        const float* inv = sm.inv + s * 128 + col0;
+        float x;
+        if (plain) {
+          x = sum_columns<kSum, false>(col, e_bias, x_mul, inv, 0);
+        } else {  // the columns this row pairs with: those that exist and are seen
+          uint64_t on = 0;
+          if (kSum) {
+            const int t = kb + lane_row;
+            for (int i = 0; i < 64; ++i) on |= (uint64_t)(t < sm.end[s * 128 + col0 + i]) << i;
+          } else {
+            const int lim = sm.end[s * 128 + lane_row] - (kb + col0);
+            on = ((uint64_t)(col0 ? mk[3] : mk[1]) << 32 | (col0 ? mk[2] : mk[0])) &
+                 (lim >= 64 ? ~0ull : lim <= 0 ? 0ull : (1ull << lim) - 1);
           }
+          x = sum_columns<kSum, true>(col, e_bias, x_mul, inv, on);
         }
         if (kSum) {
-          sum += acc.x + acc.y;
+          sum += x;
         } else if (s == 0) {
-          l[0] += acc.x + acc.y;
+          l[0] += x;
         } else {
-          l[1] += acc.x + acc.y;
+          l[1] += x;
         }
         if (kSum && s == two - 1 && col0) sm.half[buf][lane_row] = sum;
         tc::fence_before_sync();

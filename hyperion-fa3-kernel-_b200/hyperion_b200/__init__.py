@@ -81,13 +81,15 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     queued on the stream.  An outgrown block that a call under capture has used is kept:
     the graph goes on using its address."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    dev = torch.device("cuda", idx)
     key = (idx, _raw_stream(idx))
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = _workspaces.get(key)
+    if ws is not None and ws.numel() >= nbytes and not capturing:
+        return ws
     with _ws_lock:
         ws = _workspaces.get(key)
-        capturing = torch.cuda.is_current_stream_capturing()
         if ws is None or ws.numel() < nbytes:
-            new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev)
+            new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=torch.device("cuda", idx))
             if ws is not None:
                 new[:256].copy_(ws[:256])  # keep the sticky error word
                 if key in _captured:

@@ -25,6 +25,7 @@ from . import _capi, _nbytes, _raw_stream, _workspace
 _IN_DTYPES = {torch.float16: _capi.DTYPE_F16, torch.bfloat16: _capi.DTYPE_BF16, torch.float32: _capi.DTYPE_F32}
 _LAYOUTS = {"half": _capi.ROPE_HALF, "interleaved": _capi.ROPE_INTERLEAVED}
 _WS_BYTES = 1 << 16
+_I32, _F32 = torch.int32, torch.float32
 _INT_MAX = 0x7FFFFFFF
 
 
@@ -55,7 +56,7 @@ def _tables(name: str, block_tables: Optional[torch.Tensor]):
     """(address, numel) of the block tables; (None, 0) for the contiguous layout."""
     if block_tables is None or block_tables.numel() == 0:
         return None, 0
-    if not (block_tables.dtype == torch.int32):
+    if not (block_tables.dtype is _I32):
         _refuse(name, "block_tables must be int32")
     return block_tables.data_ptr(), block_tables.numel()
 
@@ -109,13 +110,14 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
     positions and pages out of range are skipped and flagged.  Two tokens of a call must
     not name the same slot or query row."""
     name = "rope_cache_write"
-    if not (Q_new.dtype in _IN_DTYPES and K_new.dtype == Q_new.dtype and V_new.dtype == Q_new.dtype):
+    dtype = Q_new.dtype
+    if not (dtype in _IN_DTYPES and K_new.dtype is dtype and V_new.dtype is dtype):
         _refuse(name, "Q_new, K_new and V_new must share a float16, bfloat16 or float32 dtype")
     if not (Q_new.dim() == 3 and K_new.dim() == 3 and V_new.shape == K_new.shape):
         _refuse(name, "Q_new must be [n_tokens, n_heads, head_dim], K_new and V_new [n_tokens, n_kv_heads, head_dim]")
     n_tokens, n_heads, head_dim = Q_new.shape
-    n_kv = K_new.shape[1]
-    if not (K_new.shape[0] == n_tokens and K_new.shape[2] == head_dim):
+    k_tokens, n_kv, k_dim = K_new.shape
+    if not (k_tokens == n_tokens and k_dim == head_dim):
         _refuse(name, "Q_new and K_new differ in tokens or head_dim")
     if not (head_dim in (128, 256)):
         _refuse(name, "head_dim must be 128 or 256")
@@ -124,21 +126,24 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
     qs, ks, vs = Q_new.stride(), K_new.stride(), V_new.stride()
     if not (n_tokens == 0 or (qs[2] == 1 and ks[2] == 1 and vs[2] == 1)):
         _refuse(name, "the dims of a head must be contiguous")
-    if not (seq_ids.dtype == torch.int32 and positions.dtype == torch.int32 and seq_ids.numel() == n_tokens
+    if not (seq_ids.dtype is _I32 and positions.dtype is _I32 and seq_ids.numel() == n_tokens
             and positions.numel() == n_tokens):
         _refuse(name, "seq_ids and positions must be int32 [n_tokens]")
-    if not (q_idx is None or (q_idx.dtype == torch.int32 and q_idx.numel() == n_tokens)):
+    if not (q_idx is None or (q_idx.dtype is _I32 and q_idx.numel() == n_tokens)):
         _refuse(name, "q_idx must be int32 [n_tokens]")
     per_head = 0
     if slots is not None:
-        per_head = 1 if slots.dim() == 2 else 0
-        if not (slots.dtype == torch.int32 and tuple(slots.shape) == ((n_tokens, n_kv) if per_head else (n_tokens,))):
+        per_head = slots.dim() - 1
+        if not (slots.dtype is _I32 and slots.shape == ((n_tokens, n_kv) if per_head else (n_tokens,))):
             _refuse(name, "slots must be int32 [n_tokens] or [n_tokens, n_kv_heads]")
     rot = n_pos = 0
     if rope is not None:
-        if not (rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[1] == 2 and rope.shape[0] >= 1):
+        if not (rope.dtype is _F32 and rope.dim() == 3):
             _refuse(name, "rope must be float32 [n_positions, 2, rotary_dim / 2]")
-        n_pos, rot = rope.shape[0], 2 * rope.shape[2]
+        n_pos, two, rot = rope.shape
+        if not (two == 2 and 1 <= n_pos <= _INT_MAX):
+            _refuse(name, "rope must be float32 [n_positions, 2, rotary_dim / 2]")
+        rot *= 2
         if not (rot <= head_dim):
             _refuse(name, "rope turns more dims than head_dim")
     if not (layout in _LAYOUTS):
@@ -147,35 +152,38 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
         _refuse(name, "seq_q must be >= 1 and fit int32")
     if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
         _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
-    if not (V_scale.dtype == torch.float32 and V_scale.numel() >= 1):
+    scales, codes = V_scale.numel(), V_cache.numel()
+    if not (V_scale.dtype is _F32 and scales >= 1):
         _refuse(name, "V_scale must be a non-empty float32 tensor")
-    if not (V_cache.element_size() == 1 and V_cache.numel() % head_dim == 0 and V_cache.numel() > 0):
+    if not (V_cache.element_size() == 1 and codes % head_dim == 0 and codes > 0):
         _refuse(name, "V_cache must hold one byte per element, [pool_rows, head_dim]")
-    pool_rows = V_cache.numel() // head_dim
-    if not (_nbytes(K_cache) >= pool_rows * head_dim // 8):
+    pool_rows = codes // head_dim
+    if not (K_cache.numel() * K_cache.element_size() >= codes // 8):
         _refuse(name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
-    if not (_nbytes(Q_words) % (head_dim // 8) == 0):
+    q_rows, rest = divmod(Q_words.numel() * Q_words.element_size(), head_dim // 8)
+    if rest:
         _refuse(name, "Q_words bytes must be a multiple of head_dim/8")
     slot_rows = 0
     if slot_positions is not None:
-        if not (slot_positions.dtype == torch.int32 and slot_positions.dim() == 2
-                and slot_positions.shape[1] == block_size * num_blocks):
+        if not (slot_positions.dtype is _I32 and slot_positions.dim() == 2):
             _refuse(name, "slot_positions must be int32 [cache rows, num_blocks * block_size]")
-        slot_rows = slot_positions.shape[0]
+        slot_rows, width = slot_positions.shape
+        if width != block_size * num_blocks:
+            _refuse(name, "slot_positions must be int32 [cache rows, num_blocks * block_size]")
     bt, bt_numel = _tables(name, block_tables)
     dev = K_cache.device
     _check_tensors(name, dev, "seq_ids positions rope block_tables V_scale Q_words K_cache V_cache q_idx slots slot_positions",
                    seq_ids, positions, rope, block_tables, V_scale, Q_words, K_cache, V_cache, q_idx, slots, slot_positions)
-    for t in (Q_new, K_new, V_new):
-        if t.device != dev:
-            _refuse(name, f"Q_new, K_new and V_new must be on {dev}")
+    idx = dev.index
+    if not (Q_new.get_device() == idx and K_new.get_device() == idx and V_new.get_device() == idx):
+        _refuse(name, f"Q_new, K_new and V_new must be on {dev}")
     args = _capi.RopeWriteArgs(
         Q_new.data_ptr(), K_new.data_ptr(), V_new.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-        _IN_DTYPES[Q_new.dtype], n_tokens, n_heads, n_kv, head_dim, rot, _LAYOUTS[layout], n_pos,
+        _IN_DTYPES[dtype], n_tokens, n_heads, n_kv, head_dim, rot, _LAYOUTS[layout], n_pos,
         rope.data_ptr() if rot else None, seq_ids.data_ptr(), positions.data_ptr(),
         None if q_idx is None else q_idx.data_ptr(), None if slots is None else slots.data_ptr(), per_head, seq_q,
-        Q_words.data_ptr(), _nbytes(Q_words) // (head_dim // 8), bt, bt_numel, block_size, num_blocks,
-        V_scale.data_ptr(), V_scale.numel(), K_cache.data_ptr(), V_cache.data_ptr(), pool_rows,
+        Q_words.data_ptr(), q_rows, bt, bt_numel, block_size, num_blocks,
+        V_scale.data_ptr(), scales, K_cache.data_ptr(), V_cache.data_ptr(), pool_rows,
         slot_positions.data_ptr() if slot_rows else None, slot_rows)
     _call(name, _capi.lib.hyperion_rope_cache_write, args, dev)
 
@@ -202,7 +210,7 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
     name = "accumulate_key_weights"
     if not (head_dim in (128, 256)):
         _refuse(name, "head_dim must be 128 or 256")
-    if not (context_lens.dtype == torch.int32):
+    if not (context_lens.dtype is _I32):
         _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
     n_q = seq_q if n_q is None else n_q
@@ -211,17 +219,18 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
     if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
         _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
     row_bytes = head_dim // 8
-    if not (_nbytes(Q) >= n_kv * kv_group * seq_q * row_bytes):
+    if not (Q.numel() * Q.element_size() >= n_kv * kv_group * seq_q * row_bytes):
         _refuse(name, "Q smaller than its rows of head_dim/8 bytes")
-    if not (_nbytes(K_cache) % row_bytes == 0 and K_cache.numel() > 0):
+    pool_rows, rest = divmod(K_cache.numel() * K_cache.element_size(), row_bytes)
+    if rest or pool_rows == 0:
         _refuse(name, "K_cache must be [pool_rows, head_dim/32] words")
     out = weights if out is None else out
-    for arg, t in (("weights", weights), ("out", out)):
-        if not (t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks):
-            _refuse(name, f"{arg} must be float32 [cache rows, >= num_blocks * block_size]")
-    if not (out.shape == weights.shape):
-        _refuse(name, "out must have the shape of weights")
-    if not (q_first is None or (q_first.dtype == torch.int32 and q_first.numel() == n_kv)):
+    shape = weights.shape
+    if not (weights.dtype is _F32 and len(shape) == 2 and shape[0] == n_kv and shape[1] >= block_size * num_blocks):
+        _refuse(name, "weights must be float32 [cache rows, >= num_blocks * block_size]")
+    if not (out is weights or (out.dtype is _F32 and out.shape == shape)):
+        _refuse(name, "out must be float32 of the shape of weights")
+    if not (q_first is None or (q_first.dtype is _I32 and q_first.numel() == n_kv)):
         _refuse(name, "q_first must be int32 [cache rows]")
     bt, bt_numel = _tables(name, block_tables)
     if not (bt_numel == 0 or bt_numel >= n_kv * num_blocks):
@@ -234,9 +243,9 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
     if n_kv == 0:
         return out
     args = _capi.KeyWeightsArgs(
-        Q.data_ptr(), K_cache.data_ptr(), _nbytes(K_cache) // row_bytes, context_lens.data_ptr(), bt, bt_numel, n_kv,
+        Q.data_ptr(), K_cache.data_ptr(), pool_rows, context_lens.data_ptr(), bt, bt_numel, n_kv,
         kv_group, seq_q, n_q, None if q_first is None else q_first.data_ptr(), head_dim, block_size, num_blocks,
-        1 if causal else 0, inv_sqrt_d, decay, weights.data_ptr(), out.data_ptr(), weights.shape[1])
+        1 if causal else 0, inv_sqrt_d, decay, weights.data_ptr(), out.data_ptr(), shape[1])
     _call(name, _capi.lib.hyperion_accumulate_key_weights, args, dev,
           _capi.lib.hyperion_key_weights_scratch_bytes(n_kv, kv_group, n_q, head_dim, block_size, num_blocks))
     return out
@@ -269,9 +278,9 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     if not (V_cache.element_size() == 1 and V_cache.dim() == 2 and V_cache.shape[1] in (128, 256) and V_cache.shape[0] > 0):
         _refuse(name, "V_cache must hold one byte per element, [pool_rows, head_dim] with head_dim 128 or 256")
     pool_rows, head_dim = V_cache.shape
-    if not (_nbytes(K_cache) >= pool_rows * head_dim // 8):
+    if not (K_cache.numel() * K_cache.element_size() >= pool_rows * head_dim // 8):
         _refuse(name, "K_cache smaller than pool_rows rows of head_dim/8 bytes")
-    if not (context_lens.dtype == torch.int32):
+    if not (context_lens.dtype is _I32):
         _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
     if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
@@ -279,16 +288,17 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     ctx_out = context_lens if context_lens_out is None else context_lens_out
     w_out = weights if weights_out is None else weights_out
     p_out = positions if positions_out is None else positions_out
-    if not (ctx_out.dtype == torch.int32 and ctx_out.numel() == n_kv):
+    if not (ctx_out.dtype is _I32 and ctx_out.numel() == n_kv):
         _refuse(name, "context_lens_out must be int32 [cache rows]")
-    for arg, t, dt in (("weights", weights, torch.float32), ("weights_out", w_out, torch.float32),
-                       ("positions", positions, torch.int32), ("positions_out", p_out, torch.int32)):
-        if not (t.dtype == dt and t.dim() == 2 and t.shape[0] == n_kv and t.shape[1] >= block_size * num_blocks
-                and t.shape == weights.shape):
-            _refuse(name, f"{arg} must be {str(dt)[6:]} [cache rows, >= num_blocks * block_size], all four of one shape")
+    shape = weights.shape
+    if not (weights.dtype is _F32 and w_out.dtype is _F32 and positions.dtype is _I32 and p_out.dtype is _I32
+            and len(shape) == 2 and shape[0] == n_kv and shape[1] >= block_size * num_blocks
+            and w_out.shape == shape and positions.shape == shape and p_out.shape == shape):
+        _refuse(name, "weights and weights_out must be float32, positions and positions_out int32, all [cache rows, >= "
+                "num_blocks * block_size] of one shape")
     keep_rows = keep if isinstance(keep, torch.Tensor) else None
     if keep_rows is not None:
-        if not (keep.dtype == torch.int32 and keep.numel() == n_kv):
+        if not (keep.dtype is _I32 and keep.numel() == n_kv):
             _refuse(name, "keep must be an int or int32 [cache rows]")
     else:
         if not (keep >= 0):
@@ -296,15 +306,17 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
         keep = min(keep, _INT_MAX)
     if not (0 <= sink <= _INT_MAX and 0 <= recent <= _INT_MAX):
         _refuse(name, "sink and recent must be >= 0 and fit int32")
-    if not (V_scale is None or (V_scale.dtype == torch.float32 and V_scale.numel() == pool_rows)):
+    if not (V_scale is None or (V_scale.dtype is _F32 and V_scale.numel() == pool_rows)):
         _refuse(name, "V_scale must be float32 [pool_rows], one scale per slot; other scales do not move")
     bt, bt_numel = _tables(name, block_tables)
     if not (bt_numel == 0 or bt_numel >= n_kv * num_blocks):
         _refuse(name, "block_tables numel < cache rows * num_blocks")
-    for arg, a, b in (("context_lens_out", context_lens, ctx_out), ("weights_out", weights, w_out),
-                      ("positions_out", positions, p_out)):
-        if a is not b:
-            _same_or_apart(name, arg, a, b)
+    if ctx_out is not context_lens:
+        _same_or_apart(name, "context_lens_out", context_lens, ctx_out)
+    if w_out is not weights:
+        _same_or_apart(name, "weights_out", weights, w_out)
+    if p_out is not positions:
+        _same_or_apart(name, "positions_out", positions, p_out)
     dev = K_cache.device
     _check_tensors(name, dev, "K_cache V_cache context_lens block_tables weights positions keep V_scale context_lens_out "
                    "weights_out positions_out", K_cache, V_cache, context_lens, block_tables, weights, positions, keep_rows,
@@ -314,7 +326,7 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     args = _capi.EvictArgs(
         K_cache.data_ptr(), V_cache.data_ptr(), None if V_scale is None else V_scale.data_ptr(), pool_rows, head_dim, n_kv,
         context_lens.data_ptr(), ctx_out.data_ptr(), bt, bt_numel, block_size, num_blocks, weights.data_ptr(),
-        w_out.data_ptr(), positions.data_ptr(), p_out.data_ptr(), weights.shape[1],
+        w_out.data_ptr(), positions.data_ptr(), p_out.data_ptr(), shape[1],
         None if keep_rows is None else keep_rows.data_ptr(), 0 if keep_rows is not None else keep, sink, recent)
     _call(name, _capi.lib.hyperion_evict_keys, args, dev,
           _capi.lib.hyperion_evict_scratch_bytes(n_kv, block_size, num_blocks))

@@ -19,10 +19,12 @@ namespace hyp {
 namespace rope {
 
 constexpr int kWarpsPerBlock = 8;
-// Query rows of one lane group in flight at once: 4 rows of 16-bit values are 128 bytes a
-// thread, enough in flight to cover HBM's latency at the kernel's occupancy.
+// Query rows of one lane group in flight at once: 64 bytes a thread and 4 blocks an SM.
+// (32768 tokens of 32 + 8 heads of 128, bf16: 98 us; 4 rows and 3 blocks 102 us, 4 rows and
+// 2 blocks 118 us, 1 row and 5 blocks 146 us: the issue slots are as busy as HBM.)
 template <typename T>
-constexpr int kUnroll = sizeof(T) == 2 ? 4 : 2;
+constexpr int kUnroll = sizeof(T) == 2 ? 2 : 1;
+constexpr int kBlocksPerSm = 4;
 
 struct Args {
   const void* q;  // [n_tokens, n_heads, D], strides in elements
@@ -116,67 +118,75 @@ __device__ __forceinline__ Run8<T> load8(const T* p) {
   return r;
 }
 
+// Eight values as pairs, for the packed f32x2 instructions (half the instructions of the
+// kernel's products and sums, which its issue slots would otherwise bound).
+struct Pairs8 {
+  float2 p[4];
+  __device__ __forceinline__ float at(int i) const { return i & 1 ? p[i / 2].y : p[i / 2].x; }
+};
+
 template <typename T>
-__device__ __forceinline__ void widen8(const Run8<T>& r, float (&f)[8]) {
-  const T* p = reinterpret_cast<const T*>(r.x);
+__device__ __forceinline__ Pairs8 widen8(const Run8<T>& r) {
+  const T* x = reinterpret_cast<const T*>(r.x);
+  Pairs8 f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = kvw::to_f32<T>(p[i]);
+  for (int i = 0; i < 4; ++i) f.p[i] = make_float2(kvw::to_f32<T>(x[2 * i]), kvw::to_f32<T>(x[2 * i + 1]));
+  return f;
 }
 
-// Signs of x*c + y*s for 8 elements as a byte (element 0 in bit 0, 1 where >= 0).  The
-// sign bits of the rounded sums are shifted in one by one; a sum that is zero or NaN sends
-// the run to the exact form.
-__device__ __forceinline__ uint32_t sign_byte(const float (&x)[8], const float (&c)[8], const float (&y)[8],
-                                              const float (&s)[8], bool minus) {
+// Signs of x*c + y*s (x*c - y*s where kMinus) for 8 elements as a byte (element 0 in bit 0, 1
+// where >= 0).  The sign bits of the rounded sums are shifted in one by one; a sum that is
+// zero or NaN sends the run to the exact form.
+template <bool kMinus>
+__device__ __forceinline__ uint32_t sign_byte(const Pairs8& x, const Pairs8& c, const Pairs8& y, const Pairs8& s) {
   uint32_t neg = 0;
   bool clear = true;
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float u = __fmul_rn(x[i], c[i]), w = __fmul_rn(y[i], s[i]);
-    const float d = minus ? __fsub_rn(u, w) : __fadd_rn(u, w);
-    neg = __funnelshift_l(__float_as_uint(d), neg, 1);
-    clear = clear && fabsf(d) > 0.f;
+  for (int i = 3; i >= 0; --i) {
+    const float2 u = __fmul2_rn(x.p[i], c.p[i]), w = __fmul2_rn(y.p[i], s.p[i]);
+    const float2 d = kMinus ? __ffma2_rn(w, make_float2(-1.f, -1.f), u) : __fadd2_rn(u, w);
+    neg = __funnelshift_l(__float_as_uint(d.y), neg, 1);
+    neg = __funnelshift_l(__float_as_uint(d.x), neg, 1);
+    clear = clear && fabsf(d.x) > 0.f && fabsf(d.y) > 0.f;
   }
   uint32_t up = ~neg & 0xFFu;
   if (!clear) {
     up = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) up |= (sum_is_nonneg(x[i], c[i], y[i], minus ? -s[i] : s[i]) ? 1u : 0u) << i;
+    for (int i = 0; i < 8; ++i) up |= (sum_is_nonneg(x.at(i), c.at(i), y.at(i), kMinus ? -s.at(i) : s.at(i)) ? 1u : 0u) << i;
   }
   return up;
 }
 
-__device__ __forceinline__ uint32_t plain_byte(const float (&x)[8]) {
+__device__ __forceinline__ uint32_t plain_byte(const Pairs8& x) {
   uint32_t up = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) up |= (x[i] >= 0.f ? 1u : 0u) << i;
+  for (int i = 0; i < 8; ++i) up |= (x.at(i) >= 0.f ? 1u : 0u) << i;
   return up;
 }
 
 // Both sign bytes of a lane's 16 dims.
 template <typename T, bool kHalf>
-__device__ __forceinline__ void turn16(const Run8<T>& r0, const Run8<T>& r1, const float (&c)[8], const float (&s)[8],
-                                       bool turned, uint32_t& b0, uint32_t& b1) {
-  float x[8], y[8];
-  widen8<T>(r0, x);
-  widen8<T>(r1, y);
+__device__ __forceinline__ void turn16(const Run8<T>& r0, const Run8<T>& r1, const Pairs8& c, const Pairs8& s, bool turned,
+                                       uint32_t& b0, uint32_t& b1) {
+  const Pairs8 x = widen8<T>(r0), y = widen8<T>(r1);
   if (!turned) {
     b0 = plain_byte(x);
     b1 = plain_byte(y);
   } else if (kHalf) {
-    b0 = sign_byte(x, c, y, s, true);
-    b1 = sign_byte(y, c, x, s, false);
+    b0 = sign_byte<true>(x, c, y, s);
+    b1 = sign_byte<false>(y, c, x, s);
   } else {
     // neighbours: members a in the even places, b in the odd ones
-    float p[8], q[8];
+    Pairs8 p, q;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = x[2 * i];
-      q[i] = x[2 * i + 1];
-      p[i + 4] = y[2 * i];
-      q[i + 4] = y[2 * i + 1];
+    for (int i = 0; i < 2; ++i) {
+      p.p[i] = make_float2(x.p[2 * i].x, x.p[2 * i + 1].x);
+      q.p[i] = make_float2(x.p[2 * i].y, x.p[2 * i + 1].y);
+      p.p[i + 2] = make_float2(y.p[2 * i].x, y.p[2 * i + 1].x);
+      q.p[i + 2] = make_float2(y.p[2 * i].y, y.p[2 * i + 1].y);
     }
-    uint32_t u = sign_byte(p, c, q, s, true), w = sign_byte(q, c, p, s, false);
+    uint32_t u = sign_byte<true>(p, c, q, s), w = sign_byte<false>(q, c, p, s);
     // bit i of u to bit 2i, of w to bit 2i + 1
     u = (u | (u << 4)) & 0x0F0Fu;
     u = (u | (u << 2)) & 0x3333u;
@@ -190,10 +200,40 @@ __device__ __forceinline__ void turn16(const Run8<T>& r0, const Run8<T>& r1, con
   }
 }
 
+// e4m3 codes of RN(v / scale), saturated, for 8 values, four a word.  v times the rounded
+// reciprocal is within 1.5 steps of the quotient, so it has the quotient's code unless a
+// border between two codes lies that near: borders have at most 5 significant bits, so the
+// low 19 bits of such a number are within 2 of 0.  Those runs, and scales whose reciprocal
+// is not an ordinary number, are divided; a scale that is a power of two never is, there
+// the product is the quotient.
+__device__ __forceinline__ void v_codes8(const Pairs8& v, float scale, float recip, uint32_t (&w)[2]) {
+  float q[8];
+  const bool ordinary = fabsf(scale) >= 0x1p-60f && fabsf(scale) <= 0x1p60f;
+  const bool power = (__float_as_uint(scale) & 0x7FFFFFu) == 0;
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 x = __fmul2_rn(v.p[i / 2], make_float2(recip, recip));
+    q[i] = x.x, q[i + 1] = x.y;
+    near = near || ((__float_as_uint(x.x) + 2) & 0x7FFFFu) <= 4 || ((__float_as_uint(x.y) + 2) & 0x7FFFFu) <= 4;
+  }
+  if (!ordinary || (near && !power)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v.at(i), scale);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint16_t lo, hi;  // the second source lands in the low byte; saturation is the clamp to +-448
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(q[4 * i + 1]), "f"(q[4 * i]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(q[4 * i + 3]), "f"(q[4 * i + 2]));
+    w[i] = (uint32_t)lo | (uint32_t)hi << 16;
+  }
+}
+
 // Warp `wid` takes token wid / parts and the row units [part * per, (part + 1) * per) of
 // its n_heads query heads and n_kv_heads (K, V) pairs.
 template <int D, typename T, bool kHalf>
-__global__ void __launch_bounds__(32 * kWarpsPerBlock, 3) rope_write_vec_kernel(Args a, int parts, int per) {
+__global__ void __launch_bounds__(32 * kWarpsPerBlock, kBlocksPerSm) rope_write_vec_kernel(Args a, int parts, int per) {
   constexpr int W = D / 32;
   constexpr int G = D / 16;  // lanes a row
   constexpr int R = 32 / G;  // rows a warp
@@ -219,15 +259,15 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock, 3) rope_write_vec_kernel(
     c0 = j;
     c1 = turning + j;
   }
-  float c[8], s[8];
+  Pairs8 c, s;
   if (turned) {
     const float4* cs = reinterpret_cast<const float4*>(a.table + (long long)pos * a.rot) + 2 * j;
     const float4* sn = reinterpret_cast<const float4*>(a.table + (long long)pos * a.rot + a.rot / 2) + 2 * j;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float4 p = __ldg(cs + i), q = __ldg(sn + i);
-      c[4 * i] = p.x, c[4 * i + 1] = p.y, c[4 * i + 2] = p.z, c[4 * i + 3] = p.w;
-      s[4 * i] = q.x, s[4 * i + 1] = q.y, s[4 * i + 2] = q.z, s[4 * i + 3] = q.w;
+      c.p[2 * i] = make_float2(p.x, p.y), c.p[2 * i + 1] = make_float2(p.z, p.w);
+      s.p[2 * i] = make_float2(q.x, q.y), s.p[2 * i + 1] = make_float2(q.z, q.w);
     }
   }
   uint8_t(*buf)[D / 8] = s_bytes[warp];
@@ -287,16 +327,11 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock, 3) rope_write_vec_kernel(
         *reinterpret_cast<uint4*>(a.k_cache + out * W + 4 * j) = *reinterpret_cast<const uint4*>(&buf[g][16 * j]);
       if (j == 0 && a.slot_positions) a.slot_positions[kv * a.pages.capacity() + slot] = pos;
       const float scale = v_scale_of(a, kv, out);
-      float x[8], y[8];
-      widen8<T>(v0, x);
-      widen8<T>(v1, y);
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i / 4] |= v_code(x[i], scale) << (8 * (i % 4));
-        w[2 + i / 4] |= v_code(y[i], scale) << (8 * (i % 4));
-      }
-      *reinterpret_cast<uint4*>(a.v_cache + out * D + 16 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+      const float recip = __frcp_rn(scale);
+      uint32_t lo[2], hi[2];
+      v_codes8(widen8<T>(v0), scale, recip, lo);
+      v_codes8(widen8<T>(v1), scale, recip, hi);
+      *reinterpret_cast<uint4*>(a.v_cache + out * D + 16 * j) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
     }
     __syncwarp();
   }

@@ -176,6 +176,44 @@ def test_rope_write_sums_next_to_zero_keep_the_exact_sign(hyperion):
     _write_check(hyperion, c)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.0, 0.25, 0.013, 3.0, 1.1, 1e-30, 1e30, float("inf"), -0.7])
+def test_rope_write_codes_on_and_next_to_the_borders(hyperion, scale, dtype):
+    """V values whose quotient by the scale is a border between two codes, or one step off it."""
+    T, D = 64, 128
+    c = _write_case(T, 2, 2, D, dtype, 64, "half", 16, 5, T, seed=1)
+    grid = torch.cat([torch.arange(0, 18) * 2.0**-10, torch.arange(16, 33)[None].mul(2.0 ** torch.arange(-10, 6)[:, None]).flatten(),
+                      torch.tensor([440.0, 448.0, 464.0, 465.0, 500.0, 1e9, float("inf")])]).float()
+    v = torch.cat([grid, -grid])[torch.arange(T * 2 * D) % (2 * grid.numel())] * scale
+    off = torch.arange(v.numel()) // (2 * grid.numel()) % 5 - 2  # steps of f32 away
+    v = torch.where(v.isfinite() & (v != 0), (v.view(torch.int32) + off.to(torch.int32)).view(torch.float32), v)
+    c.update(v=torch.nan_to_num(v, nan=0.0, posinf=3e38, neginf=-3e38).to(dtype).view(T, 2, D), scale=torch.tensor([scale]))
+    if dtype == torch.bfloat16:
+        c["v"] = c["v"].clamp(-3e38, 3e38)
+    _write_check(hyperion, c)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype, D, rot, Hq, Hk", [(torch.bfloat16, 128, 128, 32, 8), (torch.float16, 128, 96, 9, 3),
+                                                   (torch.float32, 256, 256, 5, 1), (torch.bfloat16, 256, 16, 8, 4),
+                                                   (torch.float16, 128, 0, 1, 1)])
+def test_rope_write_from_a_fused_projection(hyperion, dtype, D, rot, Hq, Hk, layout):
+    """Aligned slices of one tensor; as many tokens as fill the device, and few."""
+    h = hyperion
+    for T in (3, 700):
+        c = _write_case(T, Hq, Hk, D, dtype, rot, layout, 16, 2, T, seed=T + rot)
+        both = torch.cat([c["q"], c["k"], c["v"]], 1).to(DEV)
+        fused = [both[:, :Hq], both[:, Hq:Hq + Hk], both[:, Hq + Hk:]]
+        errors(h)
+        want, (args, kw) = _write_run(h, c, 0)
+        if T == 3:
+            for x, y in zip(want, _write_expected(c, 0)):
+                assert np.array_equal(x.cpu().numpy().view(y.dtype)[: y.shape[0]] if y.dtype == np.uint32 else x.cpu().numpy(), y)
+        got = [t.clone().zero_() if i < 3 else t.clone().fill_(-7) for i, t in enumerate(want)]
+        h.rope_cache_write(*fused, *args[3:10], got[0], got[1], got[2], **{**kw, "slot_positions": got[3]})
+        assert errors(h) == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rope_write_skips_and_flags_what_is_out_of_range(hyperion):
     c = _write_case(8, 4, 2, 128, torch.bfloat16, 64, "half", 16, 3, 8, slots="token", seed=2, max_pos=60)
     h = hyperion

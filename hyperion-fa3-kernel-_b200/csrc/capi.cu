@@ -765,13 +765,13 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
     return fail(HYPERION_ERR_INVALID_ARG, "q and k_cache must be 16-byte aligned");
   if (!aligned(x->weights, 4) || !aligned(x->weights_out, 4))
     return fail(HYPERION_ERR_INVALID_ARG, "weights and weights_out must be aligned to their element size");
-  if (x->scratch == nullptr || !aligned(x->scratch, 16))
-    return fail(HYPERION_ERR_WORKSPACE, "scratch missing or not 16-byte aligned");
   const hyp::kweights::Plan p = hyp::kweights::plan(x->n_kv, (long long)x->kv_group * x->n_q, x->head_dim,
                                                     (long long)x->block_size * x->num_blocks,
                                                     hyp::kweights::is_flat(x->inv_sqrt_d, x->head_dim));
-  if (x->scratch_bytes < p.dist_bytes + p.part_bytes)
-    return fail(HYPERION_ERR_WORKSPACE, "scratch smaller than hyperion_key_weights_scratch_bytes()");
+  const size_t need = p.dist_bytes + p.part_bytes;
+  if (need > 0 && (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16)))
+    return fail(HYPERION_ERR_WORKSPACE,
+                "scratch missing, smaller than hyperion_key_weights_scratch_bytes() or not 16-byte aligned");
   const DevInfo* di = nullptr;  // sets the kernels up on their first use on a device
   rc = get_dev(&di);
   if (rc) return rc;

@@ -140,7 +140,7 @@ __device__ __forceinline__ void store4(T* p, const T (&x)[4], int n, bool vec) {
 
 // Each thread works on 4 neighbouring slots at a time; `vec`: the rows lie on 16 bytes.
 template <int NT, int kBlocks>
-__global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster, int keys, bool vec) {
+__global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster, int keys, bool vec, bool move_here) {
   namespace cg = cooperative_groups;
   constexpr int kWarps = NT / 32;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -476,6 +476,30 @@ __global__ void __launch_bounds__(NT, kBlocks) select_kernel(Args a, int cluster
     a.counts[r] = moves;
   }
   if (cluster > 1) all.sync();  // no block leaves while another may read its counts
+  if (!move_here) return;
+  // A few moves (a step over the budget makes one): here, without a launch of their own.
+  __syncthreads();
+  const int W = a.row_words, G = 2 * W, sub = tid % G;
+  const long long row = r * a.ld;
+  for (int i = tid / G; i < moves; i += NT / G) {
+    const int dst = __ldcg(empties + i), src = __ldcg(movers + i);
+    const long long from = a.pages.slot(r, src), to = a.pages.slot(r, dst);
+    if (sub == 0) {
+      const float wv = a.w_in[row + src];
+      const int32_t pv = a.pos_in[row + src];
+      a.w_out[row + dst] = wv;
+      a.pos_out[row + dst] = pv;
+      if (a.w_out == a.w_in) a.w_out[row + src] = 0.f;
+      if (a.pos_out == a.pos_in) a.pos_out[row + src] = -1;
+    }
+    if (from < 0 || to < 0) {
+      if (sub == 0) raise_error(a.err, HYPERION_DEVERR_BAD_BLOCK);
+      continue;
+    }
+    reinterpret_cast<uint4*>(a.v)[to * G + sub] = reinterpret_cast<const uint4*>(a.v)[from * G + sub];
+    if (sub < W / 4) reinterpret_cast<uint4*>(a.k)[to * (W / 4) + sub] = reinterpret_cast<const uint4*>(a.k)[from * (W / 4) + sub];
+    if (sub == 0 && a.v_scale) a.v_scale[to] = a.v_scale[from];
+  }
 }
 
 // Moves [kMoves i, kMoves (i + 1)) of one row.  A thread looks a move's pages up; D / 16
@@ -678,6 +702,7 @@ inline size_t lists_bytes(long long n_kv, long long cap) { return (size_t)n_kv *
 inline size_t scratch_bytes(long long n_kv, long long cap) { return lists_bytes(n_kv, cap) + (size_t)n_kv * sizeof(int32_t); }
 
 constexpr size_t kMaxSmem = 227 * 1024;
+constexpr int kMovesHere = 128;    // of a row at most, that the selection makes itself
 constexpr int kBlockKeys = 16384;  // of a row per block, while 16 blocks do
 
 inline cudaError_t setup() {
@@ -720,12 +745,12 @@ inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
   auto on16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool vec = a.ld % 4 == 0 && on16(a.w_in) && on16(a.w_out) && on16(a.pos_in) && on16(a.pos_out);
   auto kernel = threads == 1024 ? select_kernel<1024, 2> : threads == 512 ? select_kernel<512, 4> : select_kernel<256, 4>;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, cluster, (int)keys, vec);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   // The most moves a row can have: its budget, or what lies beyond it.
   const long long most = a.keep_rows ? cap / 2 : std::min<long long>(a.keep, cap - a.keep);
-  if (most <= 0) return cudaSuccess;
+  const bool move_here = cluster == 1 && most <= kMovesHere;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, cluster, (int)keys, vec, move_here);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess || move_here || most <= 0) return e;
   const int moves = kMoveThreads / (2 * a.row_words) * kFlight;  // of a block
   const int per_row = (int)((most + moves - 1) / moves);
   cudaLaunchConfig_t move = {};

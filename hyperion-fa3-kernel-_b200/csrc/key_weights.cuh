@@ -176,7 +176,9 @@ __device__ __forceinline__ float warp_sum4(const float (&x)[4], int lane) {
 // A block scores kThreads * U * kSteps keys of one row.  The block's page entries, the
 // queries and E are staged in shared memory once, their global reads all in flight
 // together, so that a key costs one dependent read and few instructions of its own.
-template <int D, bool kFlat, int U, int kSteps>
+// kOne: the block has its whole row.  The distances stay in registers, the sums in shared
+// memory, and the block writes the weights itself: one launch, no scratch.
+template <int D, bool kFlat, int U, int kSteps, bool kOne>
 __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
   using DD = Dists<D>;
   using One = typename DD::One;
@@ -191,7 +193,9 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
   __shared__ uint32_t s_row[kKeys + 1];  // first pool row of each page the block touches
   __shared__ int s_best[kWarps][kBatch];
   __shared__ float s_sum[kWarps][kBatch];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ float s_inv[kBatch];
+  constexpr bool kKeep = kOne || !kFlat;  // distances are looked at again
+  if (!kOne) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / c.chunks, chunk = blockIdx.x - r * c.chunks;
   const int k0 = chunk * kKeys;
@@ -242,6 +246,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
     }
   };
 
+  float acc[kOne ? U * kSteps : 1] = {};
   for (int b = 0; b < c.batches; ++b) {
     Words<W> q[kBatch];
     int best[kBatch];
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
       best[i] = (int)DD::kOut;
     }
     Four* row = static_cast<Four*>(c.dist) + ((size_t)r * c.batches + b) * c.dist_ld + k0 + tid;
-    Four p[kFlat ? 1 : kSteps][kFlat ? 1 : U];
+    Four p[kKeep ? U * kSteps : 1];
     uint4 raw[2][U][W / 4];
     uint32_t off[2];
     fetch(raw[0], off[0], 0);
@@ -283,8 +288,8 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
         }
         Four f;
         f.x = (One)d[0], f.y = (One)d[1], f.z = (One)d[2], f.w = (One)d[3];
-        row[(step * U + u) * kThreads] = f;
-        if (!kFlat) p[kFlat ? 0 : step][kFlat ? 0 : u] = f;
+        if (!kOne) row[(step * U + u) * kThreads] = f;
+        if (kKeep) p[kKeep ? step * U + u : 0] = f;
       }
     }
     if (!kFlat) {
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
         for (int w = 0; w < kWarps; ++w) best[i] = min(best[i], s_best[w][i]);
 #pragma unroll
       for (int u = 0; u < U * kSteps; ++u) {
-        const Four f = p[kFlat ? 0 : u / U][kFlat ? 0 : u % U];
+        const Four f = p[kKeep ? u : 0];
         const uint32_t d[kBatch] = {f.x, f.y, f.z, f.w};
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
@@ -315,9 +320,39 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Args a, ChunkArgs c) {
       int m = kFlat ? 0 : (int)DD::kOut;
       if (!kFlat)
         for (int w = 0; w < kWarps; ++w) m = min(m, s_best[w][tid]);
-      c.part[((size_t)r * c.chunks + chunk) * c.batches * kBatch + b * kBatch + tid] = make_int2(m, __float_as_int(x));
+      if (kOne) {
+        s_inv[tid] = x > 0.f && b * kBatch + tid < rows ? 1.f / x : 0.f;
+      } else {
+        c.part[((size_t)r * c.chunks + chunk) * c.batches * kBatch + b * kBatch + tid] = make_int2(m, __float_as_int(x));
+      }
+    }
+    if (kOne) {
+      __syncthreads();
+      float inv[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) inv[i] = s_inv[i];
+#pragma unroll
+      for (int u = 0; u < (kOne ? U * kSteps : 0); ++u) {
+        const Four f = p[kKeep ? u : 0];
+        const uint32_t d[kBatch] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (kFlat) acc[u] = fmaf(e[d[i]], inv[i], acc[u]);
+          else if (d[i] != (One)DD::kOut) acc[u] = fmaf(e[(int)d[i] - best[i]], inv[i], acc[u]);
+        }
+      }
     }
     if (b + 1 < c.batches) __syncthreads();
+  }
+  if (kOne) {
+    const float* in = a.in + r * a.ld;
+    float* out = a.out + r * a.ld;
+    float x[kOne ? U * kSteps : 1];
+#pragma unroll
+    for (int u = 0; u < (kOne ? U * kSteps : 0); ++u) x[u] = in[min(u * kThreads + tid, last)];
+#pragma unroll
+    for (int u = 0; u < (kOne ? U * kSteps : 0); ++u)
+      if (u * kThreads + tid < n) out[u * kThreads + tid] = fmaf(a.decay, x[u], acc[u]);
   }
 }
 

@@ -768,6 +768,8 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
   const hyp::kweights::Plan p = hyp::kweights::plan(x->n_kv, (long long)x->kv_group * x->n_q, x->head_dim,
                                                     (long long)x->block_size * x->num_blocks,
                                                     hyp::kweights::is_flat(x->inv_sqrt_d, x->head_dim));
+  if ((long long)x->n_kv * std::max(p.win.chunks, 1) > 0x7fffffffLL / std::max(p.win.groups, 1))
+    return fail(HYPERION_ERR_UNSUPPORTED, "too many query rows and keys in one call");
   const size_t need = p.dist_bytes + p.part_bytes;
   if (need > 0 && (x->scratch == nullptr || x->scratch_bytes < need || !aligned(x->scratch, 16)))
     return fail(HYPERION_ERR_WORKSPACE,

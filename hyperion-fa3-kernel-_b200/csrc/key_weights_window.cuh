@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   extern __shared__ uint8_t raw[];
   auto& sm = *reinterpret_cast<WindowSmem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (!kSum) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // A block: (row, chunk) and, for the denominators, one group of queries.
   const int per_row = kSum ? c.chunks : c.chunks * c.groups;
   const int r = blockIdx.x / per_row;
@@ -186,6 +185,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
+  // Only now that every block has its tensor memory: one of the next grid, which holds some
+  // while it waits for this grid, can then not stand in the way of one of this.
+  if (!kSum) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int row = tid >> 1, half = tid & 1;  // of the expansion
   const uint32_t q_tile = smem_u32(&sm.q[0][0][0]), k_tile = smem_u32(&sm.k[0][0][0]);

@@ -263,7 +263,8 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     (keep: an int, or int32 [cache rows]).  Keys at a position below `sink` or among the
     last `recent` positions up to the row's newest rank above all others; the others rank
     by weights (float32 [cache rows, >= num_blocks * block_size], the sums of
-    accumulate_key_weights; NaN lowest); equal ranks go to the lower slot.
+    accumulate_key_weights; NaN lowest); equal ranks go to the lower slot, also among more
+    protected keys than the budget holds.
 
     Slots are not shifted: the i-th slot below m whose key goes takes the i-th kept key at
     or beyond m, so a step that drops one key moves at most one.  K words, V codes, the

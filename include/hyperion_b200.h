@@ -330,7 +330,8 @@ int hyperion_rope_cache_write(const hyperion_rope_write_args* args, void* worksp
  * weights_out is weights itself or does not overlap it.  The sum's order is fixed: the
  * same inputs give the same bits.
  * `scratch`: device memory of hyperion_key_weights_scratch_bytes() bytes, 16-byte aligned,
- * that no other call in flight uses (0 bytes: may be NULL). */
+ * that no other call in flight uses (0 bytes: may be NULL).
+ * block_size * num_blocks is at most 0x7fff0000 and pool_rows below 2^32, here and below. */
 typedef struct hyperion_key_weights_args {
   const uint32_t* q;         /* [n_kv * kv_group * seq_q, head_dim / 32] */
   const uint32_t* k_cache;   /* [pool_rows, head_dim / 32] */
@@ -359,7 +360,8 @@ int hyperion_accumulate_key_weights(const hyperion_key_weights_args* args, void*
  * m = min(n, budget) highest-ranked stay (a negative budget counts as 0).  It has no
  * counterpart in the reference.  A key is protected when its position is below `sink` or
  * above (the greatest position of the row's keys) - `recent`; protected keys rank above all
- * others, the others by `weights` (NaN lowest, -0 as 0), equal ranks by the lower slot.
+ * others, the others by `weights` (NaN lowest, -0 as 0), equal ranks by the lower slot:
+ * where more keys are protected than the budget holds, those at the lowest slots stay.
  * The i-th slot below m whose key goes takes the i-th kept key at or beyond m: K words, V
  * codes, the per-slot V scale where v_scale is given, its weight and its position.  Kept
  * keys below m stay where they are, so slots are not in the order of positions afterwards;

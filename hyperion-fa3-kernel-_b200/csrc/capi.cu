@@ -42,7 +42,7 @@ void clear_last_call() {
   for (int32_t& v : g_last_call) v = 0;
 }
 
-// A fault armed by hyperion_debug_fault for the next forward of this thread.
+// A fault armed by hyperion_debug_fault for the next forward or key weights call of this thread.
 struct FaultHook {
   bool armed = false;
   long long wait_cycles = 0;
@@ -795,6 +795,13 @@ extern "C" int hyperion_accumulate_key_weights(const hyperion_key_weights_args* 
   a.ld = x->weights_ld;
   a.stats = nullptr;
   a.err = error_word(workspace);
+  a.wait_cycles = hyp::kWaitCycles;
+  a.fault_stage = -1;
+  if (g_fault.armed) {  // consumed by this call
+    a.wait_cycles = g_fault.wait_cycles;
+    a.fault_stage = g_fault.stage;
+    g_fault.armed = false;
+  }
   const cudaError_t e = hyp::kweights::launch(a, x->head_dim, static_cast<uint8_t*>(x->scratch),
                                               static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HYPERION_OK : cuda_fail(e, "key weights launch");

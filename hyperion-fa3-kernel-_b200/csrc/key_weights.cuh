@@ -39,6 +39,8 @@ struct Args {
   long long ld;
   int2* stats;  // [n_kv * kv_group * n_q]: best popcount distance base and 1 / l
   uint32_t* err;
+  long long wait_cycles;  // bound of every device wait: kWaitCycles, shorter only under a test hook
+  int fault_stage;        // test hook: the product that blocks leave out, -1 for none
 };
 
 // E[j], j = 0..D.

@@ -55,7 +55,7 @@ struct WindowSmem {
   float half[2][128];               // sums of the upper 64 columns
   float out[kWinThreads * 8];       // the chunk's key sums (at most 16 tiles)
   int min_end;
-  alignas(8) uint64_t ready[2];
+  alignas(8) uint64_t ready[2], drain;
   uint32_t tmem_base;
   WaitCtl ctl;
 };
@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   if (tid == 0) {
     mbar_init(&sm.ready[0], 1);
     mbar_init(&sm.ready[1], 1);
+    mbar_init(&sm.drain, 1);
     sm.ctl.flag = 0;
-    sm.ctl.limit = kWaitCycles;
+    sm.ctl.limit = a.wait_cycles;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -193,8 +194,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   const uint32_t q_tile = smem_u32(&sm.q[0][0][0]), k_tile = smem_u32(&sm.k[0][0][0]);
   constexpr uint32_t kTile = D / 128 * 128 * 128;
   const uint64_t q_desc = tc::sw128_desc(q_tile, 16, 1024), k_desc = tc::sw128_desc(k_tile, 16, 1024);
-  // Thread 0: accumulator s of the tile in key buffer `buf`.
-  auto issue = [&](int s, int buf) {
+  // Thread 0: accumulator s of the tile in key buffer `buf`, the block's product `nth`.
+  auto issue = [&](int s, int buf, uint32_t nth) {
+    if (nth == (uint32_t)a.fault_stage) return;
     const uint64_t q = q_desc + (uint64_t)(s * kTile / 16), k = k_desc + (uint64_t)(buf * kTile / 16);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
@@ -225,6 +227,7 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   };
 
   uint32_t turn0 = 0, turn1 = 0;  // uses of each accumulator so far
+  bool alive = true;              // no wait of this warp ran out; thread 0 issues while it is
   const int group0 = kSum ? 0 : in_row - chunk * c.groups, group1 = kSum ? c.groups : group0 + 1;
   for (int group = group0; group < group1; ++group) {
     const int q0 = group * kWinQueries;
@@ -255,9 +258,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
     next_slot = key_slot(k0 + 2 * kWinKeys + row);
     tc::fence_proxy_async_smem();
     __syncthreads();
-    if (tid == 0) {
-      issue(0, 0);
-      if (two == 2) issue(1, 0);
+    if (tid == 0 && alive) {
+      issue(0, 0, turn0 + turn1);
+      if (two == 2) issue(1, 0, turn0 + turn1 + 1);
     }
     const int least = __reduce_min_sync(0xffffffffu, end > 0 ? end : INT_MAX);
     if (lane == 0) atomicMin(&sm.min_end, least);
@@ -292,15 +295,16 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
       float sum = 0.f;
 #pragma unroll 1
       for (int s = 0; s < two; ++s) {
-        // A wait that runs out is flagged and cuts the later ones short; what is read then is
-        // of no use, and nothing waits on it.
-        mbar_wait(&sm.ready[s], (s ? turn1 : turn0) & 1, &sm.ctl, a.err);
+        // A warp whose wait ran out reads no accumulator any more: what it holds need not be a
+        // score, and would be no place of the table.
+        alive = __all_sync(0xffffffffu, alive && mbar_wait(&sm.ready[s], (s ? turn1 : turn0) & 1, &sm.ctl, a.err));
         (s ? turn1 : turn0)++;
         tc::fence_after_sync();
         const uint32_t col = s_col + 128u * s;
         const float* inv = sm.inv + s * 128 + col0;
-        float x;
-        if (plain) {
+        float x = 0.f;
+        if (!alive) {
+        } else if (plain) {
           x = sum_columns<kSum, false>(col, e_bias, x_mul, inv, 0);
         } else {  // the columns this row pairs with: those that exist and are seen
           uint64_t on = 0;
@@ -324,9 +328,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
         if (kSum && s == two - 1 && col0) sm.half[buf][lane_row] = sum;
         tc::fence_before_sync();
         __syncthreads();
-        if (tid == 0 && g + 1 < tiles) {
+        if (tid == 0 && alive && g + 1 < tiles) {
           tc::fence_after_sync();
-          issue(s, buf ^ 1);
+          issue(s, buf ^ 1, turn0 + turn1 + two - 1);
         }
       }
       if (kSum && !col0) {
@@ -360,9 +364,9 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
       out[t] = fmaf(a.decay, in[t], w);
     }
   }
-  if (sm.ctl.flag && tid == 0) {  // let the products in flight land
-    if (turn0) mbar_drain(&sm.ready[0], (turn0 - 1) & 1, sm.ctl.limit);
-    if (turn1) mbar_drain(&sm.ready[1], (turn1 - 1) & 1, sm.ctl.limit);
+  if (tid == 0 && sm.ctl.flag) {  // let the products in flight land
+    tc::commit(&sm.drain);
+    mbar_drain(&sm.drain, 0, kWaitCycles);
   }
   tc::fence_before_sync();
   __syncthreads();

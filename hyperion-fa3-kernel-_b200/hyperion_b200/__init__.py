@@ -326,10 +326,12 @@ def read_device_errors(device=None, clear: bool = True) -> int:
 
 def debug_fault(wait_cycles: int, stage: int = -1) -> None:
     """Test hook of the bounded device waits (hyperion_debug_fault): the next forward
-    on this thread bounds every device wait by `wait_cycles` SM clocks and, for
-    stage >= 0, leaves that KV stage of its key stream unarmed so the first wait on
-    it runs out.  That forward then raises DEVERR_WAIT_TIMEOUT (read_device_errors)
-    and leaves its output incomplete; the device stays usable."""
+    or `accumulate_key_weights` on this thread bounds every device wait by
+    `wait_cycles` SM clocks and, for stage >= 0, leaves that KV stage of its key stream
+    unarmed so the first wait on it runs out (the key weights of many queries: leaves
+    out that product of each block).  That call then raises
+    DEVERR_WAIT_TIMEOUT (read_device_errors) and leaves its output incomplete; the
+    device stays usable."""
     rc = _capi.lib.hyperion_debug_fault(int(wait_cycles), int(stage))
     if rc != _capi.HYPERION_OK:
         raise RuntimeError(f"hyperion_debug_fault failed (status {rc}): {_capi.last_error()}")

@@ -416,6 +416,33 @@ def test_weights_contiguous_rows_and_a_wider_row_stride(hyperion):
     _weights_check(hyperion, c, in_place=True)
 
 
+@pytest.mark.parametrize("D, group, n_q", [(128, 2, 128), (128, 4, 100), (256, 3, 100)])
+@pytest.mark.parametrize("cycles, stage", [(2_000_000, 0), (2_000_000, 1), (2_000_000, 3), (1, -1)])
+def test_weights_of_a_window_whose_waits_run_out(hyperion, D, group, n_q, cycles, stage):
+    """No score is read after a wait that ran out: a product that never comes (the wait ends
+    after about a millisecond), or a bound too short for any, ends the call with an error flag,
+    and the next call is right.  Every block has at least four products but for the last of a
+    row, so each stage is met."""
+    c = _weights_case([700, 1500], 2, group, D=D, seq_q=n_q)
+    kw = dict(causal=True, first=(c["ctx"] - n_q).astype(np.int32), n_q=n_q)
+    args, call = _weights_check(hyperion, c, **kw)
+    hyperion.debug_fault(cycles, stage)
+    hyperion.accumulate_key_weights(*args, **call)
+    torch.cuda.synchronize()
+    err = errors(hyperion)
+    assert err == hyperion.DEVERR_WAIT_TIMEOUT or (stage < 0 and err == 0)
+    _weights_check(hyperion, c, **kw)
+
+
+def test_the_wait_hook_is_consumed_by_one_call_of_the_weights(hyperion):
+    c = _weights_case([90], 1, 1)
+    args, call = _weights_check(hyperion, c)
+    hyperion.debug_fault(2_000_000, 0)
+    hyperion.accumulate_key_weights(*args, **call)  # one query: no wait
+    assert errors(hyperion) == 0
+    _weights_check(hyperion, _weights_case([300], 1, 2, seq_q=64), n_q=64)
+
+
 def test_weights_of_no_rows(hyperion):
     w = torch.zeros(0, 16, device=DEV)
     z = torch.zeros(0, 4, dtype=i32, device=DEV)

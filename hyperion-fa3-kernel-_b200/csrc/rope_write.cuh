@@ -64,18 +64,24 @@ __device__ __forceinline__ bool sum_is_nonneg(float x, float c, float y, float s
   return __dadd_rn(__dmul_rn((double)x, (double)c), __dmul_rn((double)y, (double)s)) >= 0.0;
 }
 
+// Cache rows and query heads are int32 to the forward; beyond, the products with rows or pages
+// a head could wrap.
+constexpr long long kMaxHeads = 0x7fffffff;
+
 // Query row of (sequence b, head h) for token `tok` at `pos`, or -1.
 __device__ __forceinline__ long long q_row_of(const Args& a, int tok, int b, int pos, int h) {
   const int qi = a.q_idx ? __ldg(a.q_idx + tok) : (a.seq_q == 1 ? 0 : pos);
-  const long long row = ((long long)b * a.n_heads + h) * a.seq_q + qi;
-  return qi < 0 || qi >= a.seq_q || row >= a.q_rows ? -1 : row;
+  const long long head = (long long)b * a.n_heads + h;
+  if (head > kMaxHeads || qi < 0 || qi >= a.seq_q) return -1;
+  const long long row = head * a.seq_q + qi;
+  return row < a.q_rows ? row : -1;
 }
 
 // Pool row of cache row kv for token `tok` at `pos`, or -1 with the error raised by `flag`.
 __device__ __forceinline__ long long kv_row_of(const Args& a, int tok, int pos, int h, long long kv, bool flag, int* slot) {
   const int t = a.slots ? __ldg(a.slots + (a.slots_per_head ? (long long)tok * a.n_kv_heads + h : (long long)tok)) : pos;
   *slot = t;
-  if (t < 0 || t >= a.pages.capacity() || (a.pages.tables && kv >= a.bt_rows) ||
+  if (t < 0 || t >= a.pages.capacity() || kv > kMaxHeads || (a.pages.tables && kv >= a.bt_rows) ||
       (a.slot_positions && kv >= a.slot_rows)) {
     if (flag) raise_error(a.err, HYPERION_DEVERR_BAD_ITEM);
     return -1;

@@ -250,6 +250,26 @@ def test_rope_write_skips_and_flags_what_is_out_of_range(hyperion):
     assert flags == h.DEVERR_BAD_ITEM and bool((qw[12:16] == 0x11111111).all()) and int((sp >= 0).sum()) == 14
 
 
+@pytest.mark.parametrize("rot", [64, 38])
+@pytest.mark.parametrize("seq", [1 << 30, 1 << 29, (1 << 30) + 1, (1 << 31) - 1])
+def test_rope_write_of_a_sequence_far_beyond_the_caches(hyperion, seq, rot):
+    """Row numbers that pass 64 bits (16 heads x 2^30 rows or pages x the sequence) are out of
+    range, not row 0 or a negative one."""
+    g = torch.Generator().manual_seed(5)
+    H, D, S = 16, 128, 1 << 30
+    q, k, v = (torch.randn(1, H, D, generator=g).to(DEV) for _ in range(3))
+    rope = glue.rope_table(4, rot).to(DEV)
+    qw = torch.full((H, D // 32), 0x11111111, dtype=i32, device=DEV)
+    kc, vc = qw.clone(), torch.full((H, D), 0x11, dtype=torch.uint8, device=DEV)
+    errors(hyperion)
+    one = torch.zeros(1, dtype=i32, device=DEV)
+    for seq_q, blocks in ((S, S), (1, S), (S, 1)):
+        hyperion.rope_cache_write(q, k, v, one + seq, one, rope, None, 1, blocks, torch.ones(1, device=DEV), qw, kc, vc,
+                                  seq_q=seq_q, q_idx=one, slots=one)
+        assert errors(hyperion) & hyperion.DEVERR_BAD_ITEM
+        assert bool((qw == 0x11111111).all()) and bool((kc == 0x11111111).all()) and bool((vc == 0x11).all())
+
+
 def test_rope_write_on_another_stream_and_replayed(hyperion):
     c = _write_case(9, 8, 2, 128, torch.float16, 128, "interleaved", 16, 3, 9, seed=4)
     want = _write_expected(c, 0)

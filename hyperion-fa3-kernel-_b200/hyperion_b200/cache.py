@@ -123,6 +123,8 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
         _refuse(name, "head_dim must be 128 or 256")
     if not (n_heads >= 1 and n_kv >= 1):
         _refuse(name, "n_heads and n_kv_heads must be >= 1")
+    if not (n_tokens * (n_heads + n_kv) <= _INT_MAX):
+        _refuse(name, "too many (token, head) rows")
     qs, ks, vs = Q_new.stride(), K_new.stride(), V_new.stride()
     if not (n_tokens == 0 or (qs[2] == 1 and ks[2] == 1 and vs[2] == 1)):
         _refuse(name, "the dims of a head must be contiguous")
@@ -213,6 +215,8 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
     if not (context_lens.dtype is _I32):
         _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
+    if not (n_kv <= _INT_MAX):
+        _refuse(name, "too many cache rows")
     n_q = seq_q if n_q is None else n_q
     if not (1 <= kv_group <= _INT_MAX and 1 <= seq_q <= _INT_MAX and 1 <= n_q <= _INT_MAX):
         _refuse(name, "kv_group, seq_q and n_q must be >= 1 and fit int32")
@@ -284,6 +288,8 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
     if not (context_lens.dtype is _I32):
         _refuse(name, "context_lens must be int32")
     n_kv = context_lens.numel()
+    if not (n_kv <= _INT_MAX):
+        _refuse(name, "too many cache rows")
     if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
         _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
     ctx_out = context_lens if context_lens_out is None else context_lens_out

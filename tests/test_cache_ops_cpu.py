@@ -80,6 +80,21 @@ def test_accumulate_key_weights_refuses(hyperion, change, match):
         hyperion.accumulate_key_weights(**{**_weights_args(), **change})
 
 
+def test_counts_beyond_int32_are_refused(hyperion):
+    """Not cut to their low 32 bits: tensors without memory of their own stand for such counts."""
+    n = (1 << 32) + 4
+    x, ids = torch.zeros(1, 1, 128).expand(n, 1, 128), torch.zeros(1, dtype=i32).expand(n)
+    with pytest.raises(RuntimeError, match="too many"):
+        hyperion.rope_cache_write(**{**_write_args(), "Q_new": x, "K_new": x, "V_new": x, "seq_ids": ids, "positions": ids})
+    heads = torch.zeros(1, 1, 128).expand(3, n, 128)
+    with pytest.raises(RuntimeError, match="too many"):
+        hyperion.rope_cache_write(**{**_write_args(), "K_new": heads, "V_new": heads})
+    with pytest.raises(RuntimeError, match="too many"):
+        hyperion.accumulate_key_weights(**{**_weights_args(), "context_lens": ids})
+    with pytest.raises(RuntimeError, match="too many"):
+        hyperion.evict_keys(**{**_evict_args(), "context_lens": ids})
+
+
 def test_outputs_that_overlap_their_inputs_are_refused(hyperion):
     big = torch.zeros(9 * 32)
     with pytest.raises(RuntimeError, match="overlaps"):

@@ -110,20 +110,22 @@ __device__ __forceinline__ float sum_columns(uint32_t s_col, float e_bias, float
   constexpr uint32_t kUnit = kSum ? kUnitSum : kUnitL;
   const float kMinusTwo = __uint_as_float(0x80000002u);  // -2 x 2^-149
   float2 acc[2] = {};
+  // 16 columns are read while the 16 before them are worked on (90.0 us against 91.5 for 32
+  // read, waited for and used: 32 rows of 256 queries and up to 16384 keys).
+  uint32_t v[2][16];
+  tc::ld16(s_col, v[0]);
+  tc::ld_wait_regs(v[0]);
 #pragma unroll
-  for (int cc = 0; cc < 64; cc += 32) {
-    uint32_t v[2][16];
-    tc::ld16(s_col + cc, v[0]);
-    tc::ld16(s_col + cc + 16, v[1]);
-    tc::ld_wait_regs(v[0]);
-    tc::ld_wait_regs(v[1]);
+  for (int cc = 0; cc < 64; cc += 16) {
+    uint32_t(&now)[16] = v[cc / 16 & 1];
+    if (cc < 48) tc::ld16(s_col + cc + 16, v[(cc / 16 + 1) & 1]);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
+    for (int i = 0; i < 16; i += 4) {
       float4 scale = make_float4(1.f, 1.f, 1.f, 1.f);
       if (kSum) scale = *reinterpret_cast<const float4*>(inv + cc + i);
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
-        const float2 sc = make_float2(__uint_as_float(v[i / 16][i % 16 + j]), __uint_as_float(v[i / 16][i % 16 + j + 1]));
+        const float2 sc = make_float2(__uint_as_float(now[i + j]), __uint_as_float(now[i + j + 1]));
         float2 w;
         if (kUnit >> ((i + j) / 2 % 8) & 1) {
           const float2 x = __fmul2_rn(sc, make_float2(x_mul, x_mul));
@@ -143,6 +145,7 @@ __device__ __forceinline__ float sum_columns(uint32_t s_col, float e_bias, float
         }
       }
     }
+    if (cc < 48) tc::ld_wait_regs(v[(cc / 16 + 1) & 1]);
   }
   const float2 all = __fadd2_rn(acc[0], acc[1]);
   return all.x + all.y;
@@ -269,8 +272,13 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
       float l = 0.f;
       const int used = (n + c.tiles * kWinKeys - 1) / (c.tiles * kWinKeys);
       const float* part = c.part + ((size_t)r * c.chunks * c.groups + group) * kWinQueries + tid;
-#pragma unroll 4
-      for (int j = 0; j < used; ++j) l += __ldcg(part + (size_t)j * c.groups * kWinQueries);
+      for (int j = 0; j < used; j += 8) {  // in order, 8 reads in flight
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = j + u < used ? __ldcg(part + (size_t)(j + u) * c.groups * kWinQueries) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) l += x[u];
+      }
       sm.inv[tid] = end > 0 && l > 0.f ? 1.f / l : 0.f;
     }
     __syncthreads();

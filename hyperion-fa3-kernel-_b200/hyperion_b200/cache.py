@@ -16,8 +16,6 @@ from __future__ import annotations
 
 from typing import Optional, Union
 
-import ctypes
-
 import torch
 
 from . import _capi, _nbytes, _raw_stream, _workspace
@@ -27,6 +25,7 @@ _LAYOUTS = {"half": _capi.ROPE_HALF, "interleaved": _capi.ROPE_INTERLEAVED}
 _WS_BYTES = 1 << 16
 _I32, _F32 = torch.int32, torch.float32
 _INT_MAX = 0x7FFFFFFF
+_F32_MAX = torch.finfo(_F32).max
 
 
 def _refuse(name: str, msg: str) -> None:
@@ -53,9 +52,9 @@ def _check_tensors(name: str, dev: torch.device, names: str, *tensors: Optional[
 
 
 def _tables(name: str, block_tables: Optional[torch.Tensor]):
-    """(address, numel) of the block tables; (None, 0) for the contiguous layout."""
+    """(address, numel) of the block tables; (0, 0) for the contiguous layout."""
     if block_tables is None or block_tables.numel() == 0:
-        return None, 0
+        return 0, 0
     if not (block_tables.dtype is _I32):
         _refuse(name, "block_tables must be int32")
     return block_tables.data_ptr(), block_tables.numel()
@@ -67,16 +66,21 @@ def _same_or_apart(name: str, arg: str, a: torch.Tensor, b: torch.Tensor) -> Non
         _refuse(name, f"{arg} overlaps its input")
 
 
-def _call(name: str, fn, args, dev: torch.device, scratch: int = 0) -> None:
-    """Enqueues `fn` on the current stream of `dev`, with fresh scratch where it needs some."""
+def _scratch(dev: torch.device, nbytes: int):
+    """Fresh scratch of a call and its address (0 where it needs none)."""
+    if nbytes == 0:
+        return None, 0
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return buf, buf.data_ptr()
+
+
+def _call(name: str, fn, args: bytes, dev: torch.device) -> None:
+    """Enqueues `fn` on the current stream of `dev`."""
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            return _call(name, fn, args, dev, scratch)
-    if scratch:
-        buf = torch.empty(scratch, dtype=torch.uint8, device=dev)
-        args.scratch, args.scratch_bytes = buf.data_ptr(), scratch
+            return _call(name, fn, args, dev)
     ws = _workspace(dev, _WS_BYTES)
-    rc = fn(ctypes.byref(args), ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
+    rc = fn(args, ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
     if rc != _capi.HYPERION_OK:
         raise RuntimeError(f"{name} failed (status {rc}): {_capi.last_error()}")
 
@@ -179,14 +183,14 @@ def rope_cache_write(Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tens
     idx = dev.index
     if not (Q_new.get_device() == idx and K_new.get_device() == idx and V_new.get_device() == idx):
         _refuse(name, f"Q_new, K_new and V_new must be on {dev}")
-    args = _capi.RopeWriteArgs(
+    args = _capi.pack_rope_write(
         Q_new.data_ptr(), K_new.data_ptr(), V_new.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
         _IN_DTYPES[dtype], n_tokens, n_heads, n_kv, head_dim, rot, _LAYOUTS[layout], n_pos,
-        rope.data_ptr() if rot else None, seq_ids.data_ptr(), positions.data_ptr(),
-        None if q_idx is None else q_idx.data_ptr(), None if slots is None else slots.data_ptr(), per_head, seq_q,
+        rope.data_ptr() if rot else 0, seq_ids.data_ptr(), positions.data_ptr(),
+        0 if q_idx is None else q_idx.data_ptr(), 0 if slots is None else slots.data_ptr(), per_head, seq_q,
         Q_words.data_ptr(), q_rows, bt, bt_numel, block_size, num_blocks,
         V_scale.data_ptr(), scales, K_cache.data_ptr(), V_cache.data_ptr(), pool_rows,
-        slot_positions.data_ptr() if slot_rows else None, slot_rows)
+        slot_positions.data_ptr() if slot_rows else 0, slot_rows)
     _call(name, _capi.lib.hyperion_rope_cache_write, args, dev)
 
 
@@ -222,6 +226,8 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
         _refuse(name, "kv_group, seq_q and n_q must be >= 1 and fit int32")
     if not (block_size >= 1 and num_blocks >= 1 and block_size * num_blocks <= _INT_MAX):
         _refuse(name, "block_size and num_blocks must be >= 1, their product in int32")
+    if not (abs(inv_sqrt_d) <= _F32_MAX and abs(decay) <= _F32_MAX):
+        _refuse(name, "inv_sqrt_d and decay must be finite in float32")
     row_bytes = head_dim // 8
     if not (Q.numel() * Q.element_size() >= n_kv * kv_group * seq_q * row_bytes):
         _refuse(name, "Q smaller than its rows of head_dim/8 bytes")
@@ -246,12 +252,14 @@ def accumulate_key_weights(Q: torch.Tensor, K_cache: torch.Tensor, context_lens:
                    Q, K_cache, context_lens, block_tables, weights, out, q_first)
     if n_kv == 0:
         return out
-    args = _capi.KeyWeightsArgs(
+    nbytes = _capi.lib.hyperion_key_weights_scratch_bytes(n_kv, kv_group, n_q, head_dim, block_size, num_blocks)
+    buf, scratch = _scratch(dev, nbytes)
+    args = _capi.pack_key_weights(
         Q.data_ptr(), K_cache.data_ptr(), pool_rows, context_lens.data_ptr(), bt, bt_numel, n_kv,
-        kv_group, seq_q, n_q, None if q_first is None else q_first.data_ptr(), head_dim, block_size, num_blocks,
-        1 if causal else 0, inv_sqrt_d, decay, weights.data_ptr(), out.data_ptr(), shape[1])
-    _call(name, _capi.lib.hyperion_accumulate_key_weights, args, dev,
-          _capi.lib.hyperion_key_weights_scratch_bytes(n_kv, kv_group, n_q, head_dim, block_size, num_blocks))
+        kv_group, seq_q, n_q, 0 if q_first is None else q_first.data_ptr(), head_dim, block_size, num_blocks,
+        1 if causal else 0, inv_sqrt_d, decay, weights.data_ptr(), out.data_ptr(), shape[1],
+        scratch, nbytes)
+    _call(name, _capi.lib.hyperion_accumulate_key_weights, args, dev)
     return out
 
 
@@ -330,11 +338,12 @@ def evict_keys(K_cache: torch.Tensor, V_cache: torch.Tensor, context_lens: torch
                    V_scale, ctx_out, w_out, p_out)
     if n_kv == 0:
         return ctx_out
-    args = _capi.EvictArgs(
-        K_cache.data_ptr(), V_cache.data_ptr(), None if V_scale is None else V_scale.data_ptr(), pool_rows, head_dim, n_kv,
+    nbytes = _capi.lib.hyperion_evict_scratch_bytes(n_kv, block_size, num_blocks)
+    buf, scratch = _scratch(dev, nbytes)
+    args = _capi.pack_evict(
+        K_cache.data_ptr(), V_cache.data_ptr(), 0 if V_scale is None else V_scale.data_ptr(), pool_rows, head_dim, n_kv,
         context_lens.data_ptr(), ctx_out.data_ptr(), bt, bt_numel, block_size, num_blocks, weights.data_ptr(),
         w_out.data_ptr(), positions.data_ptr(), p_out.data_ptr(), shape[1],
-        None if keep_rows is None else keep_rows.data_ptr(), 0 if keep_rows is not None else keep, sink, recent)
-    _call(name, _capi.lib.hyperion_evict_keys, args, dev,
-          _capi.lib.hyperion_evict_scratch_bytes(n_kv, block_size, num_blocks))
+        0 if keep_rows is None else keep_rows.data_ptr(), 0 if keep_rows is not None else keep, sink, recent, scratch, nbytes)
+    _call(name, _capi.lib.hyperion_evict_keys, args, dev)
     return ctx_out

@@ -80,6 +80,24 @@ def test_accumulate_key_weights_refuses(hyperion, change, match):
         hyperion.accumulate_key_weights(**{**_weights_args(), **change})
 
 
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan"), 1e39, -1e300])
+@pytest.mark.parametrize("arg", ["inv_sqrt_d", "decay"])
+def test_scales_that_are_not_finite_in_float32_are_refused(hyperion, arg, value):
+    with pytest.raises(RuntimeError, match="finite"):
+        hyperion.accumulate_key_weights(**{**_weights_args(), arg: value})
+
+
+@pytest.mark.parametrize("cls, pack", [("RopeWriteArgs", "pack_rope_write"), ("KeyWeightsArgs", "pack_key_weights"),
+                                       ("EvictArgs", "pack_evict")])
+def test_packed_arguments_are_the_structures_bytes(hyperion, cls, pack):
+    from hyperion_b200 import _capi
+    args = getattr(_capi, cls)
+    values = [0.37 + i if t is ctypes.c_float else 1 + i * 7 for i, (_, t) in enumerate(args._fields_)]
+    back = args.from_buffer_copy(getattr(_capi, pack)(*values))
+    for (name, t), v in zip(args._fields_, values):
+        assert getattr(back, name) == (np.float32(v) if t is ctypes.c_float else v), name
+
+
 def test_counts_beyond_int32_are_refused(hyperion):
     """Not cut to their low 32 bits: tensors without memory of their own stand for such counts."""
     n = (1 << 32) + 4

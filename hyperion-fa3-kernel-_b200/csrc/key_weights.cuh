@@ -130,6 +130,11 @@ __device__ __forceinline__ void load_query(Words<W>& q, const Args& a, long long
 // Where 2 |inv_sqrt_d| D <= 80 (kFlat; 22.6 for 1 / sqrt(128)) no exponential reaches the
 // clamp whatever the row's best score, so E is taken relative to distance 0.  Otherwise a
 // chunk's sum is relative to the chunk's best distance, which is stored with it.
+//
+// 512 rows of 2048 to 8192 keys of 128 dims, 4 queries each: 31 us for both, 42 MB of keys
+// and 21 MB of sums read or written (2 TB/s).  About 110 instructions per 32 keys and 4
+// queries, 12 of them POPC, keep the issue slots 60 % busy.  One kernel with a cluster per
+// row, the sums exchanged over distributed shared memory: 40 us, for its cluster barriers.
 // ---------------------------------------------------------------------------
 constexpr int kBatch = 4;       // queries scored together against a key
 constexpr int kMaxBatches = 4;  // of one call on this path: 16 queries
@@ -474,7 +479,9 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(Args a, ChunkArgs c, int 
 
 // ---------------------------------------------------------------------------
 // Many queries at a scale beyond kFlat: two kernels on the CUDA cores, with each query's
-// best and 1 / l between them.  (At the usual scales: key_weights_window.cuh.)
+// best and 1 / l between them.  (At the usual scales: key_weights_window.cuh.)  Every pair's
+// popcount is taken three times, from words in L1: 32 rows of 256 queries and up to 16384
+// keys 940 us, where the tensor-core form takes 90.
 // ---------------------------------------------------------------------------
 // One block per query row: the least distance and the sum of E over its keys.
 template <int D>

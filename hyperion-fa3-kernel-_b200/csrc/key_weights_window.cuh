@@ -24,6 +24,12 @@
 // The two accumulators of a key tile (128 columns each, two blocks on an SM) are computed
 // and read in turn: while the threads read one, the tensor core fills the other, and the
 // next tile's sign bits, loaded at the start of a turn, are expanded at its end.
+//
+// 32 rows of 256 queries and up to 16384 keys of 128 dims: 90 us for both kernels, where the
+// products alone would take 15 at the bf16 rate and the bytes 1.5.  What bounds them is the
+// exponentials (the table alone 97 us, the unit alone 119), a block's setup (40 % of its time
+// at 4 tiles a chunk; 8 tiles leave SMs without work) and 16 warps an SM.  512 threads a
+// block, one on an SM: 122 us.
 #pragma once
 
 #include "key_weights.cuh"

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock, kBlocksPerSm) rope_write_
 // ---------------------------------------------------------------------------
 // The scalar kernel: any even rotary_dim, any alignment and stride.  One warp per (token,
 // query head) and per (token, KV head); lane l takes dims l, l + 32, ..., so a ballot is
-// one sign word.
+// one sign word.  (32768 tokens of 32 + 8 heads of 128, bf16: 625 us, the vector kernel 98.)
 // ---------------------------------------------------------------------------
 template <int D, typename T>
 __global__ void __launch_bounds__(32 * kWarpsPerBlock) rope_write_kernel(Args a) {

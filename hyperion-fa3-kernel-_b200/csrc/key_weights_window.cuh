@@ -203,8 +203,11 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
   const uint32_t q_tile = smem_u32(&sm.q[0][0][0]), k_tile = smem_u32(&sm.k[0][0][0]);
   constexpr uint32_t kTile = D / 128 * 128 * 128;
   const uint64_t q_desc = tc::sw128_desc(q_tile, 16, 1024), k_desc = tc::sw128_desc(k_tile, 16, 1024);
-  // Thread 0: accumulator s of the tile in key buffer `buf`, the block's product `nth`.
+  // Thread 0, behind a barrier: accumulator s of the tile in key buffer `buf`, the block's
+  // product `nth`.  The fence orders it after the accumulator's reads by every warp, which
+  // lie before the barrier.
   auto issue = [&](int s, int buf, uint32_t nth) {
+    tc::fence_after_sync();
     if (nth == (uint32_t)a.fault_stage) return;
     const uint64_t q = q_desc + (uint64_t)(s * kTile / 16), k = k_desc + (uint64_t)(buf * kTile / 16);
 #pragma unroll
@@ -342,10 +345,7 @@ __global__ void __launch_bounds__(kWinThreads, D == 128 ? 2 : 1) window_kernel(A
         if (kSum && s == two - 1 && col0) sm.half[buf][lane_row] = sum;
         tc::fence_before_sync();
         __syncthreads();
-        if (tid == 0 && alive && g + 1 < tiles) {
-          tc::fence_after_sync();
-          issue(s, buf ^ 1, turn0 + turn1 + two - 1);
-        }
+        if (tid == 0 && alive && g + 1 < tiles) issue(s, buf ^ 1, turn0 + turn1 + two - 1);
       }
       if (kSum && !col0) {
         float* out = sm.out + g * kWinKeys + lane_row;

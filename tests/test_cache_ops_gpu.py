@@ -395,6 +395,17 @@ def test_weights_windows_over_many_tiles_and_chunks(hyperion, D, group, n_q, cau
     _weights_check(hyperion, c, causal=causal, first=first, n_q=n_q, err=hyperion.DEVERR_BAD_BLOCK)
 
 
+@pytest.mark.parametrize("D, group, lens", [(128, 1, [1000, 600, 257]), (128, 3, [700, 1, 513]), (256, 2, [900, 256, 301])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_whole_prompts_of_many_groups_over_many_chunks(hyperion, D, group, lens, causal):
+    """Every row of the prompts (n_q left out): up to nine groups of 256 queries, whose
+    products follow one another in the same accumulators, over chunks of 256 keys, among them
+    chunks that no query of a group sees."""
+    c = _weights_case(lens, 1, group, D, seq_q=max(lens), seed=group + D)
+    _weights_check(hyperion, c, causal=causal, decay=0.5)
+    _weights_check(hyperion, c, causal=causal, in_place=True)
+
+
 @pytest.mark.parametrize("D", [128, 256])
 def test_weights_many_rows_of_short_and_long_contexts(hyperion, D):
     """Enough keys for the blocks of many keys a thread, ends inside and between them."""

@@ -551,6 +551,37 @@ int hyperion_reset_counter(void* workspace, size_t workspace_bytes, void* stream
   return HYPERION_OK;
 }
 
+int hyperion_workspace_alloc(size_t bytes, void** workspace) {
+  if (workspace == nullptr) return fail(HYPERION_ERR_INVALID_ARG, "workspace is NULL");
+  if (bytes < hyp::kWsPartials) return fail(HYPERION_ERR_INVALID_ARG, "a workspace has at least 256 bytes");
+  // Relaxed for these calls alone: another stream of the process may be under capture.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+  void* d = nullptr;
+  cudaStream_t st = nullptr;
+  const char* where = "cudaMalloc(workspace)";
+  e = cudaMalloc(&d, bytes);
+  if (e == cudaSuccess) {
+    where = "cudaStreamCreateWithFlags";
+    e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  }
+  if (e == cudaSuccess) {
+    where = "cudaMemsetAsync(workspace)";
+    e = cudaMemsetAsync(d, 0, bytes, st);
+  }
+  if (e == cudaSuccess) {
+    where = "cudaStreamSynchronize";
+    e = cudaStreamSynchronize(st);
+  }
+  if (st != nullptr) cudaStreamDestroy(st);
+  if (e != cudaSuccess && d != nullptr) cudaFree(d);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cuda_fail(e, where);
+  *workspace = d;
+  return HYPERION_OK;
+}
+
 int hyperion_read_device_errors(void* workspace, size_t workspace_bytes, void* stream, uint32_t* flags,
                                 int32_t clear) {
   if (workspace == nullptr || workspace_bytes < hyp::kWsPartials || flags == nullptr)

@@ -62,7 +62,7 @@ _KERNELS = {1: "row", 2: "group", 3: "group_mma", 4: "tile"}
 _ws_lock = threading.Lock()
 _workspaces: dict = {}
 _captured: set = set()  # keys of workspaces that a captured graph may hold the address of
-_retired: list = []  # outgrown workspaces of those keys: a graph replays on them
+_retired: dict = {}  # key: outgrown workspaces that are still used or hold unread flags
 
 
 def _raw_stream(idx: int) -> int:
@@ -70,7 +70,24 @@ def _raw_stream(idx: int) -> int:
     return torch._C._cuda_getCurrentRawStream(idx)
 
 
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+class _FixedBlock:
+    """A zeroed workspace from the library, kept for the life of the process."""
+
+    def __init__(self, nbytes: int):
+        ptr = ctypes.c_void_p()
+        rc = _capi.lib.hyperion_workspace_alloc(nbytes, ctypes.byref(ptr))
+        if rc != _capi.HYPERION_OK:
+            raise RuntimeError(f"hyperion_workspace_alloc failed (status {rc}): {_capi.last_error()}")
+        self._ptr, self._nbytes = ptr.value, nbytes
+
+    def data_ptr(self) -> int:
+        return self._ptr
+
+    def numel(self) -> int:
+        return self._nbytes
+
+
+def _workspace(device: torch.device, nbytes: int):
     """Workspace (work counter, error word, split-KV partials) of the current stream of
     `device`, grown on demand.
 
@@ -79,7 +96,9 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     ordered by its stream.  It is allocated on that stream as well, so when it grows
     the caching allocator hands the old block out again only after the work already
     queued on the stream.  An outgrown block that a call under capture has used is kept:
-    the graph goes on using its address."""
+    the graph goes on using its address.  A block first needed under capture comes from
+    the library: torch's would be the graph's own memory, which its other scratch may
+    have used before, and the fill would only run with the graph, and then each time."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     key = (idx, _raw_stream(idx))
     capturing = torch.cuda.is_current_stream_capturing()
@@ -89,11 +108,13 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
-            new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=torch.device("cuda", idx))
+            nbytes = max(nbytes, 1 << 16)
+            new = _FixedBlock(nbytes) if capturing else torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", idx))
             if ws is not None:
-                new[:256].copy_(ws[:256])  # keep the sticky error word
-                if key in _captured:
-                    _retired.append(ws)
+                if capturing or key in _captured:
+                    _retired.setdefault(key, []).append(ws)  # read_device_errors looks there too
+                else:
+                    new[:256].copy_(ws[:256])  # keep the sticky error word
             ws = new
             _workspaces[key] = ws
         if capturing:
@@ -312,16 +333,21 @@ def hyperion_reset_counter(*, grid=None, block=None, device=None) -> None:
 def read_device_errors(device=None, clear: bool = True) -> int:
     """Synchronises the current stream of `device` and returns the DEVERR_* flags that
     the calls issued on that stream raised (each stream has its own workspace and so
-    its own error word)."""
+    its own error word).  The calls of a CUDA graph raise theirs, on every replay and
+    whatever stream that runs on, in the workspace of the stream they were captured on:
+    wait for the replay, then read with that stream current."""
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index)
     with torch.cuda.device(dev):
-        ws = _workspace(dev, 1 << 16)
-        flags = ctypes.c_uint32(0)
-        rc = _capi.lib.hyperion_read_device_errors(ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream,
-                                                   ctypes.byref(flags), 1 if clear else 0)
-    if rc != _capi.HYPERION_OK:
-        raise RuntimeError(f"hyperion_read_device_errors failed (status {rc}): {_capi.last_error()}")
-    return int(flags.value)
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        found = 0
+        for ws in (_workspace(dev, 1 << 16), *_retired.get((dev.index, stream), ())):
+            flags = ctypes.c_uint32(0)
+            rc = _capi.lib.hyperion_read_device_errors(ws.data_ptr(), ws.numel(), stream, ctypes.byref(flags),
+                                                       1 if clear else 0)
+            if rc != _capi.HYPERION_OK:
+                raise RuntimeError(f"hyperion_read_device_errors failed (status {rc}): {_capi.last_error()}")
+            found |= int(flags.value)
+    return found
 
 
 def debug_fault(wait_cycles: int, stage: int = -1) -> None:

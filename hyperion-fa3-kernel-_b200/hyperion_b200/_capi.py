@@ -40,6 +40,7 @@ PATH_TILE = 2
 # Every symbol include/hyperion_b200.h declares.
 EXPORTED = (
     "hyperion_workspace_bytes",
+    "hyperion_workspace_alloc",
     "hyperion_apex_kernel",
     "hyperion_apex_kernel_ex",
     "hyperion_reset_counter",
@@ -181,6 +182,8 @@ def _load() -> ctypes.CDLL:
     lib = ctypes.CDLL(LIB_PATH)
     lib.hyperion_workspace_bytes.restype = ctypes.c_size_t
     lib.hyperion_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32]
+    lib.hyperion_workspace_alloc.restype = ctypes.c_int
+    lib.hyperion_workspace_alloc.argtypes = [ctypes.c_size_t, ctypes.POINTER(_vp)]
     lib.hyperion_apex_kernel.restype = ctypes.c_int
     lib.hyperion_apex_kernel.argtypes = _FWD_ARGS + [_vp, ctypes.c_size_t, _vp]
     lib.hyperion_apex_kernel_ex.restype = ctypes.c_int

@@ -171,6 +171,13 @@ int hyperion_apex_kernel_ex(const int32_t* worklist, int32_t total_work,
  * on its own stream, and this call zeroes it explicitly (asynchronous on `stream`). */
 int hyperion_reset_counter(void* workspace, size_t workspace_bytes, void* stream);
 
+/* Device memory for a workspace on the current device, zeroed when the call returns, in
+ * *workspace; release it with cudaFree once no call and no captured graph uses it.  Unlike
+ * cudaMalloc and a fill on a stream that is being captured, it may be called during a
+ * capture (of any mode), and nothing of it becomes part of the graph: a fill that replays
+ * would clear the error word each time. */
+int hyperion_workspace_alloc(size_t bytes, void** workspace);
+
 /* Test hook for the bounded device waits; it has no counterpart in the reference,
  * whose kernel waits without a bound.  Arms a fault for the next forward or
  * hyperion_accumulate_key_weights issued on this host thread (hyperion_apex_kernel,

@@ -421,6 +421,36 @@ def test_weights_scales_of_either_sign_and_beyond_the_clamp(hyperion, inv, seq_q
     _weights_check(hyperion, _weights_case([77, 400], 2, 4, seq_q=seq_q, seed=9), inv=inv)
 
 
+@pytest.mark.parametrize("inv", [1.0, -3.0, 1e4])
+@pytest.mark.parametrize("D, group", [(128, 3), (256, 5)])
+@pytest.mark.parametrize("rows", [5, 250])
+def test_weights_beyond_the_clamp_over_many_chunks(hyperion, rows, D, group, inv):
+    """The two launches of few queries, each chunk's sum relative to its own best score: one key
+    a thread (5 rows) and eight (250); lengths inside a chunk, no key, one, and a chunk whose
+    pages all lie outside the pool."""
+    h = hyperion
+    lens = ([2500, 1, 0, 2100, 300] * 50)[:rows]
+    c = _weights_case(lens, 1, group, D, block=64, seed=rows + D)
+    assert c["block"] * c["nb"] > 2048
+    _weights_check(h, c, inv=inv, decay=0.5)
+    c["table"][0, : 32 if rows > 5 else 8] = -1
+    c["table"][3, 32] = 1 << 30
+    _weights_check(h, c, inv=inv, err=h.DEVERR_BAD_BLOCK)
+    c = _weights_case(lens[:5] + [2500] * (rows - 5), 1, group, D, block=64, seq_q=2500, seed=D)
+    _weights_check(h, c, inv=inv, causal=True, first=(c["ctx"] - 3).astype(np.int32), n_q=3)
+
+
+@pytest.mark.parametrize("D, inv", [(128, 1.0), (256, -3.0)])
+def test_weights_of_causal_windows_beyond_the_clamp(hyperion, D, inv):
+    h = hyperion
+    c = _weights_case([400, 33, 1, 0, 270], 1, 2, D, seq_q=400, seed=D)
+    first = (c["ctx"] - 40).astype(np.int32)
+    _weights_check(h, c, inv=inv, causal=True, first=first, n_q=40, decay=0.5)
+    c["table"][0, :3], c["table"][4, 16] = -1, 1 << 30
+    _weights_check(h, c, inv=inv, causal=True, first=first, n_q=40, err=h.DEVERR_BAD_BLOCK)
+    _weights_check(h, c, inv=inv, causal=True, err=h.DEVERR_BAD_BLOCK)  # the first rows see no key
+
+
 def test_weights_repeated_keys_and_exact_matches(hyperion):
     c = _weights_case([300], 2, 4, seed=1)
     c["k"][::3] = c["q"][0]
@@ -581,6 +611,21 @@ def test_evict_page_sizes_and_row_budgets(hyperion, block, nb, D, slot_scale):
 @pytest.mark.parametrize("in_place", [True, False])
 def test_evict_long_rows(hyperion, lens, keep, in_place):
     _evict_check(hyperion, _evict_case(lens, block=64, seed=keep), keep, 4, 100, in_place=in_place)
+
+
+@pytest.mark.parametrize("capacity", [803200, 820032])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_capacities_around_the_most_that_sixteen_blocks_hold(hyperion, capacity, in_place):
+    """16 blocks a row of 50,208 keys, nearly all their shared memory, and one block a row
+    beyond.  Budgets among ties, below the protected keys and above the length; a bad page."""
+    h = hyperion
+    c = _evict_case([capacity - 31, 700, 0], block=64, nb=capacity // 64, seed=capacity, slot_scale=True)
+    _evict_check(h, c, [capacity - 20000, 650, 5], 4, 100, in_place=in_place)  # 10 % of the sums are 0
+    c["table"][0, 12000:12050], c["table"][0, 1] = -1, 1 << 30  # pages of sources, one of destinations
+    _evict_check(h, c, [5000, 40, 0], 0, 64, err=h.DEVERR_BAD_BLOCK, in_place=in_place)
+    _evict_check(h, c, 50, 2, 2**31 - 1, in_place=in_place)  # all protected: nothing moves
+    c["w"][0, ::7], c["w"][0, 1::9] = np.nan, -np.inf
+    _evict_check(h, c, 700000, 4, 100, err=h.DEVERR_BAD_BLOCK, in_place=in_place)  # among the NaN
 
 
 def test_evict_ties_infinities_nan_and_signed_zeros(hyperion):

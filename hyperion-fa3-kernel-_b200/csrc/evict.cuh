@@ -66,12 +66,15 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 //      each warp writes its slots' places into the row's two lists (slots that empty below
 //      m, keys that move), in slot order.
 //
-// move_kernel: the moves of all rows, 128 a block, whichever row they belong to.
+// move_kernel: the moves of all rows, 128 a block (64 at head_dim 256), whichever row they
+// belong to.
 //
 // 128 rows of 32768 keys cut to 4096: selection 35 us, 34 MB of sums and positions, bound by
 // its instructions (54 % of the issue slots) and barriers; moves 31 us, scattered rows of 128,
 // 16 and 4 bytes, 147 MB of DRAM traffic at 4.5 TB/s.  Both in one kernel: 158 us, since a
-// row's moves are then one SM's.  512 rows of 4097 cut to 4096: 25 us.
+// row's moves are then one SM's.  512 rows of 4097 cut to 4096: 25 us.  The instances of 512
+// and 1024 threads are held to 32 registers for their blocks an SM and spill (104 and 44
+// bytes of stores a thread).
 // ---------------------------------------------------------------------------
 constexpr int kBins = 4096;  // two 16-bit counts a word: a block has at most 52k keys
 constexpr int kBinBits = 12;
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(Args a, int blocks_p
 // ---------------------------------------------------------------------------
 // Rows too long for 16 blocks' shared memory (from about 800,000 keys): one block a row, which
 // reads the ranks anew for each turn.  8 rows of 131072, which do not need it: 1137 us, the
-// clusters 46.
+// clusters 46.  8 rows of 820,032: 6.6 ms, where clusters take 0.16 for rows of 803,200.
 // ---------------------------------------------------------------------------
 constexpr int kLongThreads = 1024;
 
@@ -708,7 +711,11 @@ inline size_t lists_bytes(long long n_kv, long long cap) { return (size_t)n_kv *
 inline size_t scratch_bytes(long long n_kv, long long cap) { return lists_bytes(n_kv, cap) + (size_t)n_kv * sizeof(int32_t); }
 
 constexpr size_t kMaxSmem = 227 * 1024;
-constexpr int kMovesHere = 128;    // of a row at most, that the selection makes itself
+// Moves of a row at most, that the selection makes itself: no launch of their own, but one
+// block's.  512 rows cut to 4096 by 1 key: 20.2 us here, 21.3 by move_kernel; by 64: 22.6 both;
+// by 128: 25.7 and 23.9; by 512: 53 and 39.  64 rows: 13.4 and 14.4, 14.6 and 14.8, 17.2 and
+// 14.7, 28 and 14.
+constexpr int kMovesHere = 128;
 constexpr int kBlockKeys = 16384;  // of a row per block, while 16 blocks do
 
 inline cudaError_t setup() {
@@ -728,7 +735,8 @@ inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
   int cluster = 1;
   auto part = [&](int c) { return ((cap + c - 1) / c + 31) / 32 * 32; };
   while (cluster < kMaxCluster && part(cluster) > kBlockKeys) cluster *= 2;
-  // Few rows: more blocks a row while the device has room and a block keeps 4096 keys.
+  // Few rows: more blocks a row while the device has room and a block keeps 4096 keys.  Not 16:
+  // 8 rows of 131072 take 89 us with clusters of 16, 36 with 8; 4 rows 59 and 34.
   while (cluster < 8 && (long long)a.n_kv * cluster * 2 <= n_sm && part(cluster) >= 8192) cluster *= 2;
   const long long keys = part(cluster);
   const size_t smem = sizeof(Shared) + (size_t)keys * 4 + (size_t)keys / 32 * 8;
@@ -736,6 +744,12 @@ inline cudaError_t launch(const Args& a, int n_sm, cudaStream_t st) {
     evict_long_kernel<<<(unsigned)a.n_kv, kLongThreads, 0, st>>>(a);
     return cudaGetLastError();
   }
+  // Threads by the keys of a block.  Rows that fill the device, cut by one key and to a quarter,
+  // us with 256 / 512 / 1024 threads: 2049 keys 25 / 28 / 44 and 53 / 57 / 68, 4097 20 / 23 / 34
+  // and 47 / 49 / 60, 5001 22.7 / 23.6 / 31 and 48 / 48 / 57, 6001 26.1 / 25.7 / 34 and
+  // 51 / 49 / 57, 8192 27 / 23 / 26 and 60 / 57 / 51, 12289 36 / 30 / 33 and 68 / 63 / 56,
+  // 16384 40 / 28 / 24 and 64 / 53 / 51: 512 overtake 256 between 5000 and 6000 keys, 1024
+  // overtake 512 from 8192 on, first where many keys go.
   const int threads = keys > 8192 ? 1024 : keys > 4608 ? 512 : 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)a.n_kv * cluster));

@@ -132,9 +132,12 @@ __device__ __forceinline__ void load_query(Words<W>& q, const Args& a, long long
 // chunk's sum is relative to the chunk's best distance, which is stored with it.
 //
 // 512 rows of 2048 to 8192 keys of 128 dims, 4 queries each: 31 us for both, 42 MB of keys
-// and 21 MB of sums read or written (2 TB/s).  About 110 instructions per 32 keys and 4
-// queries, 12 of them POPC, keep the issue slots 60 % busy.  One kernel with a cluster per
-// row, the sums exchanged over distributed shared memory: 40 us, for its cluster barriers.
+// and 21 MB of sums read or written (2 TB/s).  By the counters 155 warp instructions per 32
+// keys and 4 queries in the scores, 12 of them POPC, and 63 in the sums: 15 us of the 31 if
+// every issue slot were used, and 50 to 60 % are.  The rest is short blocks (8 keys a thread
+// behind a prologue of page entries, queries and the table), barriers, and one kernel after
+// the other.  One kernel with a cluster per row, the sums exchanged over distributed shared
+// memory: 40 us, for its cluster barriers.
 // ---------------------------------------------------------------------------
 constexpr int kBatch = 4;       // queries scored together against a key
 constexpr int kMaxBatches = 4;  // of one call on this path: 16 queries

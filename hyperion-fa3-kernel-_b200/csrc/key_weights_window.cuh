@@ -30,6 +30,12 @@
 // exponentials (the table alone 97 us, the unit alone 119), a block's setup (40 % of its time
 // at 4 tiles a chunk; 8 tiles leave SMs without work) and 16 warps an SM.  512 threads a
 // block, one on an SM: 122 us.
+//
+// Every tile of a row is computed for every group, also where causal queries see none of it:
+// whole prompts (4 sequences of 8 KV heads, 4 query heads each) 0.23 ms at 1024 rows, 0.58 at
+// 2048, 2.2 at 4096; without the mask 0.18, 0.46 and 1.8.  Fewer query rows than 128 leave
+// columns that hold no query but are computed: 64 rows of 8192 keys with 32 queries 69 us, with
+// 16, by the popcount kernels, 22.
 #pragma once
 
 #include "key_weights.cuh"
@@ -428,7 +434,8 @@ inline Plan plan(long long n_kv, long long rows, int head_dim, long long cap, bo
   p.flat = flat;
   p.few = rows <= kMaxBatches * kBatch;
   if (!p.few && flat) {
-    // Chunks of up to 16 tiles, shorter ones while they leave SMs without blocks (2 each).
+    // Chunks of up to 16 tiles, shorter ones while the sums have fewer than 4 blocks an SM: two
+    // rounds of the 2 that an SM holds at head_dim 128, four of the 1 at head_dim 256.
     p.win.groups = (int)((rows + kWinQueries - 1) / kWinQueries);
     p.win.tiles = kMaxChunkTiles;
     while (p.win.tiles > 2 && n_kv * ((cap + p.win.tiles * kWinKeys - 1) / (p.win.tiles * kWinKeys)) < 4 * kSms) p.win.tiles /= 2;

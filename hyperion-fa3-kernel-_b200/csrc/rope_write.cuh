@@ -21,7 +21,8 @@ namespace rope {
 constexpr int kWarpsPerBlock = 8;
 // Query rows of one lane group in flight at once: 64 bytes a thread and 4 blocks an SM.
 // (32768 tokens of 32 + 8 heads of 128, bf16: 98 us; 4 rows and 3 blocks 102 us, 4 rows and
-// 2 blocks 118 us, 1 row and 5 blocks 146 us: the issue slots are as busy as HBM.)
+// 2 blocks 118 us, 1 row and 5 blocks 146 us: the issue slots are as busy as HBM.  At the 64
+// registers of 4 blocks every instance spills, 84 to 116 bytes of stores a thread.)
 template <typename T>
 constexpr int kUnroll = sizeof(T) == 2 ? 2 : 1;
 constexpr int kBlocksPerSm = 4;

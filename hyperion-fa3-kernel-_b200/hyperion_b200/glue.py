@@ -119,7 +119,9 @@ def rope_table(n_positions: int, rotary_dim: int, base: float = 10000.0, *, scal
                 the factor, the fastest not at all;
       "bands"   pairs that turn more than high_turns times over original_positions stay,
                 those that turn less than low_turns times are divided by the factor, those
-                between go linearly from one to the other in their number of turns."""
+                between go linearly from one to the other in their number of turns.
+    Tables of trained models differ in these limits and in what the ramp is linear in; a ramp
+    in turns, as here, often ends at high_turns 4."""
     if n_positions < 1 or rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("n_positions must be >= 1 and rotary_dim even and >= 2")
     if not base > 0 or not factor > 0:

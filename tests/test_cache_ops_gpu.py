@@ -580,6 +580,31 @@ def _evict_check(h, c, keep, sink=0, recent=0, err=0, in_place=True):
         assert np.array_equal(t["scale"].cpu().numpy(), scale)
 
 
+@pytest.mark.parametrize("lens, keep", [([300, 64, 0, 129], 100), ([5000, 900, 4096], 1000), ([40000, 3], 30000)])
+@pytest.mark.parametrize("apart", [("weights",), ("positions",), ("context_lens",), ("weights", "context_lens")])
+def test_evict_with_some_outputs_in_place(hyperion, lens, keep, apart):
+    """Each output by itself is its input or another tensor."""
+    h, c = hyperion, _evict_case(lens, block=16, seed=keep)
+    t = {n: gpu(c[n]) for n in ("k", "v", "ctx", "table", "w", "pos")}
+    of = {"weights": "w", "positions": "pos", "context_lens": "ctx"}
+    outs = {n + "_out": torch.full_like(t[of[n]], -9) for n in apart}
+    errors(h)
+    new = h.evict_keys(t["k"], t["v"], t["ctx"], t["table"], c["block"], c["nb"], t["w"], t["pos"], keep, sink=4, recent=20,
+                       **outs)
+    assert errors(h) == 0
+    k, v, _, ctx, w, pos = evict(c["k"], c["v"], None, c["ctx"], c["table"], c["block"], c["nb"], c["w"], c["pos"], keep, 4, 20)
+    assert np.array_equal(u32(t["k"]), k) and np.array_equal(t["v"].cpu().numpy(), v)
+    assert np.array_equal(new.cpu().numpy(), ctx)
+    for n, want in (("weights", w), ("positions", pos), ("context_lens", ctx)):
+        got = outs[n + "_out"] if n in apart else t[of[n]]
+        if n in apart:
+            assert np.array_equal(t[of[n]].cpu().numpy(), c[of[n]])  # the input stays
+            for r, length in enumerate(c["ctx"]):
+                if n != "context_lens":
+                    want[r, length:] = -9  # and nothing is written beyond the row
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
 LENS = [0, 1, 2, 16, 31, 33, 200, 511]
 
 
